@@ -440,6 +440,124 @@ typedef struct {
 } tidal_prefill_args;
 int tidal_prefill(const tidal_prefill_args* args, void* stream);
 
+/* ---------------------------------------------------------- 8-bit KV cache
+ * A second form of the KV pool: codes in e4m3 (4 exponent and 3 mantissa bits, no infinity, largest value 448),
+ * layout [pages][2][page_size][Hkv][D] as above, one byte per element; and one power-of-two scale per (block of
+ * `block` consecutive slots of a page, plane, KV head): scales [pages][2][page_size / block][Hkv], a byte b that
+ * stands for 2^(b-127) (b = 0: the block reads as zeros).  The value of an element is code * scale.  No counterpart
+ * in the reference, whose pools hold the model's type.
+ *
+ * tidal_append_kv8 quantises the K,V of new tokens into their slots.  A block's scale is the smallest 2^e, e >= -126,
+ * with max|x| <= 448 * 2^e over the finite elements of its tokens, and never shrinks while the block fills: if tokens
+ * behind its first slot are appended to a block whose stored scale is smaller, the codes already there are moved to the
+ * new scale (code * 2^(e_old - e), nearest even; exact unless that leaves e4m3's normal range); the block's first slot
+ * starts its scale afresh.  Elements are rounded to the nearest e4m3 value, ties to even; infinities become +-448 * 2^e,
+ * NaN stays NaN.  Token i belongs to sequence b = i / tokens_per_seq, cache slot pos0[b] + i % tokens_per_seq.
+ * Two sequences of one call must not share a page that is appended to.  f16, bf16 or f32 rows, D 64 or 128. */
+typedef struct {
+    const void* d_k;             /* [batch * tokens_per_seq] rows of [Hkv][D], k_stride elements apart */
+    const void* d_v;
+    int64_t k_stride, v_stride;  /* multiples of 8 (16-bit types) or 4 (f32) */
+    void* d_kv;                  /* codes */
+    uint8_t* d_scales;
+    const int32_t* d_page_table; /* as in tidal_attn_args */
+    int64_t page_table_stride;
+    const int32_t* d_pos0;       /* [batch] int32 device, or NULL: every sequence starts at slot pos0 */
+    int32_t pos0;
+    int32_t batch, tokens_per_seq, num_kv_heads, head_dim, page_size, block, dtype;
+    int64_t num_pages;           /* a slot or page outside the pool is skipped and TIDAL_DEV_BAD_INDEX OR-ed into *d_status */
+    uint32_t* d_status;          /* optional */
+} tidal_append_kv8_args;
+int tidal_append_kv8(const tidal_append_kv8_args* args, void* stream);
+
+/* Slots [start, stop) of every sequence of an 8-bit pool as rows of dtype: d_out [batch][stop - start][2][Hkv][D] — per
+ * sequence a 16/32-bit pool of page_size 1, as tidal_prefill takes it.  f16 saturates at +-65504.  With d_seq_lens,
+ * rows at and behind a sequence's length are left as they were; so are rows whose page lies outside the pool
+ * (TIDAL_DEV_BAD_INDEX in *d_status). */
+typedef struct {
+    const void* d_kv;
+    const uint8_t* d_scales;
+    const int32_t* d_page_table;
+    int64_t page_table_stride;
+    const int32_t* d_seq_lens;   /* [batch], or NULL: all slots up to stop are read */
+    void* d_out;
+    int32_t start, stop;
+    int32_t batch, num_kv_heads, head_dim, page_size, block, dtype;
+    int64_t num_pages;
+    uint32_t* d_status;
+} tidal_read_kv8_args;
+int tidal_read_kv8(const tidal_read_kv8_args* args, void* stream);
+
+/* One decode step of attention over an 8-bit pool: tidal_decode_attention's full, selection and sparse layers
+ * (o = softmax(q K^T sm_scale) V, one new query per sequence), the codes read as they are stored.  Scores, softmax
+ * statistics and sums are fp32.  A sequence or list without tokens gives o = 0, lse = -inf.
+ * d_scores receives the natural-scale logits (column = token position, or the entry's place in its list; columns
+ * beyond a list's length are left as they were), d_lse the natural log of the softmax denominator.  A list entry or
+ * page out of range is skipped as if it were not listed (its logits column is left as it was) and
+ * TIDAL_DEV_BAD_INDEX is recorded in the workspace. */
+typedef struct {
+    const void* d_q;             /* [batch][Hq][D] of dtype */
+    void* d_o;                   /* [batch][Hq][D] of dtype */
+    const void* d_kv;
+    const uint8_t* d_scales;
+    const int32_t* d_page_table;
+    int64_t page_table_stride;
+    const int32_t* d_seq_lens;   /* [batch] or NULL: all = seq_len */
+    int32_t seq_len;             /* host-side upper bound of (and default for) the lengths */
+    const int32_t* d_sel_idx;    /* [batch][sel_rows][sel_stride] token positions, or NULL: all tokens */
+    int32_t sel_rows, sel_count; /* sel_rows 1 or Hq */
+    int64_t sel_stride;
+    const int32_t* d_sel_counts; /* NULL, or [batch][sel_rows] valid entries per list */
+    float* d_scores;             /* NULL, or [batch][Hq][score_stride] */
+    int64_t score_stride;
+    float* d_lse;                /* NULL, or [batch][Hq] */
+    int32_t batch, num_qo_heads, num_kv_heads, head_dim, page_size, block, dtype;
+    int64_t num_pages;
+    float sm_scale;              /* <= 0: 1/sqrt(D) */
+} tidal_attn_kv8_args;
+int tidal_decode_attention_kv8(const tidal_attn_kv8_args* args, void* d_ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------- bounding a cache by attention weight
+ * What a token has been worth to the queries so far: w[b][j] = decay * w[b][j] + sum_h exp(s[b][h][j] - lse[b][h])
+ * for j < length, from the logits and log-sum-exps that a selection layer writes (any attention call of this library
+ * with per-head logits).  The heads are summed in a fixed order.  Columns at and behind the length are left as they
+ * were; lse = -inf (a row without tokens) contributes nothing. */
+typedef struct {
+    const float* d_scores;       /* [batch][heads][score_stride] */
+    int64_t score_stride;
+    const float* d_lse;          /* [batch][heads] */
+    float* d_weights;            /* [batch][weight_stride], updated in place */
+    int64_t weight_stride;
+    const int32_t* d_seq_lens;   /* [batch] or NULL: all = seq_len */
+    int32_t seq_len;             /* upper bound of (and default for) the lengths */
+    int32_t batch, heads;
+    float decay;
+} tidal_weights_args;
+int tidal_accumulate_weights(const tidal_weights_args* args, void* stream);
+
+/* Drops the pages of least weight from a page table, for every row whose sequence uses more than keep_pages pages:
+ * the first sink_pages and the last recent_pages (>= 1: the last page may be partly filled) stay, and of the pages
+ * between them those of greatest weight, until keep_pages are left.  A page's weight is the sum of its tokens' weights,
+ * formed in 64 bits and rounded to fp32; equal weights go to the lower page, NaN counts as the greatest.  Written to
+ * the outputs, which must not overlap the inputs: the table row with the kept pages first (in order) and the dropped
+ * ones behind them (in order: the next pages this sequence grows into, or the caller's to hand out again), entries
+ * behind the pages in use as they were; the weights of the kept tokens moved along, zeros behind them up to the old
+ * length, the rest of the max_len columns as they were; the new lengths.  Rows within keep_pages are copied.  No K or V
+ * is touched: attention does not depend on the order of the tokens it attends to. */
+typedef struct {
+    const float* d_weights;      /* [rows][weight_stride] */
+    float* d_weights_out;
+    int64_t weight_stride;       /* of both */
+    const int32_t* d_page_table; /* [rows][page_table_stride] */
+    int32_t* d_page_table_out;
+    int64_t page_table_stride;   /* of both */
+    const int32_t* d_seq_lens;   /* [rows], or NULL: all = max_len */
+    int32_t* d_seq_lens_out;     /* [rows] */
+    int32_t max_len;             /* upper bound of the lengths */
+    int32_t rows, page_size, keep_pages, sink_pages, recent_pages;
+} tidal_evict_args;
+int tidal_evict_pages(const tidal_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

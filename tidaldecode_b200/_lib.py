@@ -21,6 +21,7 @@ XCHG_MAX_CTAS = 64
 EXPORTS = (
     "tidal_version", "tidal_last_error", "tidal_launch_count", "tidal_ws_bytes", "tidal_ws_init", "tidal_ws_release", "tidal_ws_status",
     "tidal_decode_attention", "tidal_plan_chunks", "tidal_topk", "tidal_topk_static", "tidal_topk_static_status", "tidal_rope_append", "tidal_update_page_meta", "tidal_estimate", "tidal_merge_partials", "tidal_merge_partials_strided", "tidal_rms_norm", "tidal_decode_linear", "tidal_decode_qkv", "tidal_peer_all_gather", "tidal_peer_exchange_reset", "tidal_prefill",
+    "tidal_append_kv8", "tidal_read_kv8", "tidal_decode_attention_kv8", "tidal_accumulate_weights", "tidal_evict_pages",
 )
 
 
@@ -121,6 +122,57 @@ class PrefillArgs(C.Structure):
     ]
 
 
+class AppendKv8Args(C.Structure):
+    _fields_ = [
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+        ("d_kv", C.c_void_p), ("d_scales", C.c_void_p), ("d_page_table", C.c_void_p), ("page_table_stride", C.c_int64),
+        ("d_pos0", C.c_void_p), ("pos0", C.c_int32),
+        ("batch", C.c_int32), ("tokens_per_seq", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("block", C.c_int32), ("dtype", C.c_int32),
+        ("num_pages", C.c_int64), ("d_status", C.c_void_p),
+    ]
+
+
+class ReadKv8Args(C.Structure):
+    _fields_ = [
+        ("d_kv", C.c_void_p), ("d_scales", C.c_void_p), ("d_page_table", C.c_void_p), ("page_table_stride", C.c_int64),
+        ("d_seq_lens", C.c_void_p), ("d_out", C.c_void_p), ("start", C.c_int32), ("stop", C.c_int32),
+        ("batch", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("block", C.c_int32), ("dtype", C.c_int32),
+        ("num_pages", C.c_int64), ("d_status", C.c_void_p),
+    ]
+
+
+class AttnKv8Args(C.Structure):
+    _fields_ = [
+        ("d_q", C.c_void_p), ("d_o", C.c_void_p), ("d_kv", C.c_void_p), ("d_scales", C.c_void_p),
+        ("d_page_table", C.c_void_p), ("page_table_stride", C.c_int64),
+        ("d_seq_lens", C.c_void_p), ("seq_len", C.c_int32),
+        ("d_sel_idx", C.c_void_p), ("sel_rows", C.c_int32), ("sel_count", C.c_int32), ("sel_stride", C.c_int64),
+        ("d_sel_counts", C.c_void_p), ("d_scores", C.c_void_p), ("score_stride", C.c_int64), ("d_lse", C.c_void_p),
+        ("batch", C.c_int32), ("num_qo_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("block", C.c_int32), ("dtype", C.c_int32),
+        ("num_pages", C.c_int64), ("sm_scale", C.c_float),
+    ]
+
+
+class WeightsArgs(C.Structure):
+    _fields_ = [
+        ("d_scores", C.c_void_p), ("score_stride", C.c_int64), ("d_lse", C.c_void_p), ("d_weights", C.c_void_p),
+        ("weight_stride", C.c_int64), ("d_seq_lens", C.c_void_p), ("seq_len", C.c_int32),
+        ("batch", C.c_int32), ("heads", C.c_int32), ("decay", C.c_float),
+    ]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [
+        ("d_weights", C.c_void_p), ("d_weights_out", C.c_void_p), ("weight_stride", C.c_int64),
+        ("d_page_table", C.c_void_p), ("d_page_table_out", C.c_void_p), ("page_table_stride", C.c_int64),
+        ("d_seq_lens", C.c_void_p), ("d_seq_lens_out", C.c_void_p), ("max_len", C.c_int32),
+        ("rows", C.c_int32), ("page_size", C.c_int32), ("keep_pages", C.c_int32), ("sink_pages", C.c_int32), ("recent_pages", C.c_int32),
+    ]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -175,6 +227,12 @@ def _load() -> C.CDLL:
     lib.tidal_peer_exchange_reset.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
     lib.tidal_prefill.restype = C.c_int
     lib.tidal_prefill.argtypes = [C.POINTER(PrefillArgs), C.c_void_p]
+    for name, args in (("tidal_append_kv8", AppendKv8Args), ("tidal_read_kv8", ReadKv8Args),
+                       ("tidal_accumulate_weights", WeightsArgs), ("tidal_evict_pages", EvictArgs)):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
+    lib.tidal_decode_attention_kv8.restype = C.c_int
+    lib.tidal_decode_attention_kv8.argtypes = [C.POINTER(AttnKv8Args), C.c_void_p, C.c_size_t, C.c_void_p]
     return lib
 
 
