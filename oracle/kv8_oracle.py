@@ -66,15 +66,17 @@ def append(kv: torch.Tensor, scales: torch.Tensor, k: torch.Tensor, v: torch.Ten
                     scales[pg, plane, at // block, h] = e + 127
 
 
-def attention(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, sm: float):
-    """One query row q [D] over K,V [n,D] (float64): (o, logits, lse, sum_j p_j |v_j|, max_j sum_d |q_d k_jd| sm)."""
+def attention(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, sm: float, vscale: torch.Tensor | None = None):
+    """One query row q [D] over K,V [n,D] (float64): (o, logits, lse, sum_j p_j |v_j|, max_j sum_d |q_d k_jd| sm) and, with
+    the values' scales [n], max_j (p_j scale_j) * sum_j |v_j| / scale_j."""
     if K.shape[0] == 0:
         z = torch.zeros(q.shape[0], dtype=torch.float64)
-        return z, torch.zeros(0, dtype=torch.float64), -math.inf, z.clone(), 0.0
+        return (z, torch.zeros(0, dtype=torch.float64), -math.inf, z.clone(), 0.0) + (() if vscale is None else (z.clone(),))
     x = K @ q.double() * sm
     lse = torch.logsumexp(x, 0)
     p = torch.exp(x - lse)
-    return p @ V, x, float(lse), p @ V.abs(), float((K.abs() @ q.double().abs()).max() * sm)
+    got = p @ V, x, float(lse), p @ V.abs(), float((K.abs() @ q.double().abs()).max() * sm)
+    return got if vscale is None else got + ((p * vscale).max() * (V.abs() / vscale[:, None]).sum(0),)
 
 
 def accumulate(scores, lse, weights, lens, decay):

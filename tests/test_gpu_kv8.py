@@ -7,6 +7,9 @@ A = sum_j p_j |v_j| and x the logits, a computed output may be off by
                                            steps are t * eps(type) wide whatever |o|, so at least t * eps(type)/2
     2 * dx * A                             logits off by dx change every weight and the denominator by a factor 1 +- dx
     2^-11 A (16-bit types) or 2^-21 A      weights enter the product with V rounded to 11 (or twice 11) bits
+    2^-38 U                                fp16's steps end at 2^-24, and weights are scaled so that the largest p_j 2^ev_j of
+                                           the tokens lies in (2^13, 2^14]: a weight is off by 2^-25 at least, that is by up to
+                                           2^-38 of the largest; U = max_j (p_j 2^ev_j) * sum_j |code_j|
     (n/4 + 32) * 2^-23 * A                 fp32 sums over n tokens, at least four to an addition, each step off by 2^-23
 with dx = 20 * 2^-23 * max_j sum_d |q_d k_jd| sm (8 to 16 fp32 additions of exact products, the scale factors) plus
 2^-22 * (2 + max|x| * log2 e) for the exponential and its argument.  Logits themselves are held to that dx."""
@@ -229,12 +232,13 @@ def _attention_case(T, dt, B, Hq, Hkv, D, lens, page, block, lists="all", k=0, c
                 n = k if counts is None else counts[b]
                 pos = sel[b, 0 if lists == "shared" else h, :n].long()
             pg = table[b].long()[pos // page]
-            want, x, z, A, dot = K8.attention(q[b, h], vals[pg, 0, pos % page, h // G], vals[pg, 1, pos % page, h // G], sm)
+            vs = 2.0 ** (scales[pg, 1, pos % page // block, h // G].double() - 127)
+            want, x, z, A, dot, U = K8.attention(q[b, h], vals[pg, 0, pos % page, h // G], vals[pg, 1, pos % page, h // G], sm, vs)
             n = pos.numel()
             top = float(x.abs().max()) if n else 0.0
             dx = 20 * 2.0 ** -23 * dot
             de = dx + 2.0 ** -22 * (2 + top * LOG2E)
-            tol = eps * want.abs() + A * (2 * de + (2.0 ** -21 if dt == "f32" else 2.0 ** -11) + (n / 4 + 32) * 2.0 ** -23)
+            tol = eps * want.abs() + A * (2 * de + (2.0 ** -21 if dt == "f32" else 2.0 ** -11) + (n / 4 + 32) * 2.0 ** -23) + 2.0 ** -38 * U
             tol = torch.maximum(tol, torch.full_like(tol, torch.finfo(dtype).smallest_normal * eps) + tol - eps * want.abs())
             most = torch.finfo(dtype).max * (1 + eps)                    # from here on a result of the type is infinite
             over = want.abs() - tol >= most

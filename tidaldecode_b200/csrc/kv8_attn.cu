@@ -1,7 +1,40 @@
-// One decode step of attention over an 8-bit KV pool.
+// One decode step of attention over an 8-bit KV pool, on the tensor cores (mma.sync m16n8k16, fp16 operands).
+//
+// The mathematics.  A cached element is code * 2^e with one e per (block of slots, head), so e4m3 codes go into the
+// products as fp16 values (exactly: fp16 holds every e4m3 value) and the scales stay outside:
+//     x_j = (q . k_j) 2^(ek_j) sm log2(e)                       logits in log2 units
+//     l   = sum_j 2^(x_j - m)                                   m >= all x_j so far
+//     O   = sum_j 2^(x_j + ev_j - M) v_j                        M >= all x_j + ev_j so far
+// The value scale goes into the exponent of the weight that the product with V uses, and that weight has a maximum of its
+// own: a token of great weight and tiny values does not push the others' weights out of fp16.  m and M are rounded up
+// to integers, so x - m and x + ev - M are single roundings and rescaling multiplies by exact powers of two.
+//
+// Rounding choices.  q is scaled by a power of two so that its largest element lies in [2^11, 2^12): fp16 then holds
+// bf16 and fp16 rows exactly (elements 2^25 below the largest lose bits); fp32 rows are split into two fp16 terms (22
+// bits).  Weights are scaled to at most 2^14 (tokens down to 2^-38 of the heaviest still count) and rounded to fp16: half a
+// step is 2^-12, next to 2^-9 for a bf16 result; for fp16 and fp32 results a second fp16 term carries the remainder.
+// Accumulators, maxima and sums are fp32.
+//
+// Data movement.  The order of the contraction index and of the output elements is free as long as both operands agree, so
+// every lane copies exactly the bytes that its own fragments need (cp.async, 16 bytes at a time) into a ring of
+// shared memory that no other lane reads: no barrier, no bank conflict, no register held by data in flight.  With
+// lane = 4 g + t, a tile of 16 tokens:
+//     S = Q K^T  (M = heads, N = tokens): lane holds 64-byte pieces t*16.. of K rows g and 8+g; the four bytes of one
+//                word are elements 2t, 2t+1, 2t+8, 2t+9 of a k-step
+//     O^T = V^T P^T  (M = elements, N = heads): lane holds bytes g*D/8.. of V rows 2t, 2t+1, 2t+8, 2t+9, and the
+//                accumulator of S already has the layout of the B operand P^T
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace tidal {
+
+constexpr int kKv8Warps = 8;
+constexpr int kKv8Tile = 16;             // tokens a warp takes at a time
+constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself
 
 struct AttnKv8Params {
     const void* q;
@@ -18,115 +51,514 @@ struct AttnKv8Params {
     float* scores;
     int64_t score_stride;
     float* lse;
-    float* part_o;               // [B * Hq][chunks][D]
-    float* part_ml;              // [B * Hq][chunks][2]
+    float* part_o;               // [slices][ctas + lists][HC * rows][D]
+    float* part_ml;              // [slices][ctas + lists][HC * rows][2]
+    uint32_t* arrivals;          // [lists * slices][16], zero at rest
     uint32_t* status;
-    int32_t Hq, Hkv, G, block, chunks;
+    int32_t Hq, Hkv, G, block;
+    int32_t lists, per_head;     // token lists: one per sequence, or one per (sequence, query head)
+    int32_t groups, rows;        // query heads of a KV head are taken `rows` (at most 16) at a time, in `groups` groups
+    int32_t HC, slices;          // (KV head, group) units per CTA; CTAs along the units
+    int32_t ctas;                // CTAs that share the lists' tiles
+    int32_t ragged;              // lengths differ: 1 = they are added up by every CTA, 2 = a CTA per list
+    int32_t tiles_per_list;      // ragged == 0
+    int32_t page_shift, block_shift;     // -1 where the size is no power of two
     float sm_scale;
 };
 
-constexpr int kKv8Warps = 4;
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8(void* dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One CTA per (query head, chunk of its token list); a warp takes every fourth token, its lanes the elements.
-template <typename T, int D>
-__global__ void __launch_bounds__(kKv8Warps * 32) attn_kv8_kernel(const AttnKv8Params p) {
-    constexpr int EPL = D / 32;
-    __shared__ float sh_o[kKv8Warps][D];
-    __shared__ float sh_ml[kKv8Warps][2];
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 codes to two fp16 pairs.
+__device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The part of (lo, hi) that `packed` lost, again as fp16.
+__device__ __forceinline__ uint32_t pack_f16_rest(float lo, float hi, uint32_t packed) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+    return pack_f16(lo - f.x, hi - f.y);
+}
+
+__device__ __forceinline__ int list_len_kv8(const AttnKv8Params& p, int list) {
+    if (p.sel_idx) return p.sel_counts ? max(0, min(p.sel_counts[list], p.sel_count)) : p.sel_count;
+    return p.seq_lens ? max(0, min(p.seq_lens[list], p.seq_len)) : p.seq_len;
+}
+
+template <int D>
+struct Kv8Ring {
+    static constexpr int stages = D == 128 ? 3 : 5;
+    static constexpr int stage_bytes = kKv8Tile * 2 * D;                 // of one warp: K rows, then V rows
+    static constexpr size_t bytes = (size_t)kKv8Warps * stages * stage_bytes;
+};
+// Four consecutive elements of a row.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* f) {
+    if (sizeof(T) == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = to_f32(e[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+    if (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = v;
+    } else {
+        const T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+    }
+}
+
+template <typename T, int D, bool R2>    // R2: more than 8 query heads to a unit
+__global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
+    constexpr bool QS = sizeof(T) == 4, PS = !std::is_same<T, __nv_bfloat16>::value;
+    constexpr int S = Kv8Ring<D>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t sc_ring[kKv8Warps][S][kKv8Tile];                 // per token: K scale byte, valid, V scale byte
+    __shared__ float ml[kKv8Warps][16][2];
+    __shared__ int s_scan[kKv8Warps + 1];
+    __shared__ int s_last;
+    int* prefix = reinterpret_cast<int*>(smem + Kv8Ring<D>::bytes);    // [lists + 1] when the lengths are added up here
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int TG = kKv8Warps / p.HC, TT = kKv8Tile * TG;
+    const int uw = warp % p.HC, tg = warp / p.HC;
+    const int cta = blockIdx.x, slice = blockIdx.y;
+    unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D>::stage_bytes;
+
     pdl_wait();
     pdl_launch_dependents();
-    const int chunk = blockIdx.x, hq = blockIdx.y % p.Hq, b = blockIdx.y / p.Hq;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = hq / p.G;
-    const int seq = p.seq_lens ? max(0, min(p.seq_lens[b], p.seq_len)) : p.seq_len;
-    const size_t list = p.sel_rows == 1 ? b : (size_t)b * p.Hq + hq;
-    int n = seq;
-    if (p.sel_idx) n = p.sel_counts ? max(0, min(p.sel_counts[list], p.sel_count)) : p.sel_count;
-    const int per = (n + p.chunks - 1) / p.chunks;
-    const int t0 = chunk * per, t1 = min(n, t0 + per);
-    float q[EPL];
-    const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)b * p.Hq + hq) * D + lane * EPL;
+
+    // ---- this CTA's range of tiles
+    int64_t tile, tile_end;
+    int total;
+    if (p.ragged == 0) {
+        total = p.tiles_per_list * p.lists;
+    } else if (p.ragged == 1) {
+        const int per = (p.lists + blockDim.x - 1) / blockDim.x, first = tid * per;
+        int sum = 0;
+        for (int i = first; i < min(first + per, p.lists); ++i) sum += max(1, (list_len_kv8(p, i) + TT - 1) / TT);
+        int incl = sum;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) q[i] = to_f32(qrow[i]);
-    float m = -INFINITY, l = 0.f, o[EPL] = {};
-    for (int t = t0 + warp; t < t1; t += kKv8Warps) {
-        const int pos = p.sel_idx ? p.sel_idx[list * p.sel_stride + t] : t;
-        int entry = 0;
-        int64_t page = pos >= seq ? -1 : p.map.page_of(b, pos, &entry);
-        if (page < 0) {
-            if (lane == 0) atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
-            continue;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += y;
         }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        int at = incl - sum;
+        for (int i = 0; i < warp; ++i) at += s_scan[i];
+        for (int i = first; i < min(first + per, p.lists); ++i) {
+            prefix[i] = at;
+            at += max(1, (list_len_kv8(p, i) + TT - 1) / TT);
+            if (i == p.lists - 1) prefix[p.lists] = at;
+        }
+        __syncthreads();
+        total = prefix[p.lists];
+    } else {
+        total = p.lists;
+    }
+    const int ctas = min(p.ctas, total);                                 // no CTA without a tile: every part that is waited for comes
+    if (cta >= ctas) return;
+    auto cta_begin = [&](int c) -> int { return (int)((int64_t)c * total / ctas); };
+    auto cta_of = [&](int tl) -> int { return (int)((((int64_t)tl + 1) * ctas - 1) / total); };       // the CTA whose range holds the tile
+    tile = p.ragged == 2 ? cta : cta_begin(cta);
+    tile_end = p.ragged == 2 ? cta + 1 : cta_begin(cta + 1);
+    int list = 0;
+    if (p.ragged == 0) {
+        list = tile < total ? (int)(tile / p.tiles_per_list) : 0;
+    } else if (p.ragged == 1) {
+        int lo = 0, hi = p.lists;                                        // last list that starts at or before the tile
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= tile) lo = mid; else hi = mid;
+        }
+        list = lo;
+    } else {
+        list = cta;
+    }
+
+    for (; tile < tile_end; ++list) {
+        // ---- the segment of `list` that lies in this CTA's range: entries [tok0, tok1)
+        const int len = list_len_kv8(p, list);
+        int first_tile, n_tiles;
+        if (p.ragged == 0) first_tile = list * p.tiles_per_list, n_tiles = p.tiles_per_list;
+        else if (p.ragged == 1) first_tile = prefix[list], n_tiles = prefix[list + 1] - first_tile;
+        else first_tile = list, n_tiles = 1;
+        const int seg_end = (int)min(tile_end, (int64_t)first_tile + n_tiles);
+        const bool whole = p.ragged == 2 || (tile == first_tile && seg_end == first_tile + n_tiles);
+        const int tok0 = p.ragged == 2 ? 0 : (int)min((int64_t)len, (tile - first_tile) * TT);
+        const int tok1 = p.ragged == 2 ? len : (int)min((int64_t)len, (int64_t)(seg_end - first_tile) * TT);
+        const int n_it = (tok1 - tok0 + TT - 1) / TT;
+
+        const int b = p.per_head ? list / p.Hq : list;
+        const int unit = slice * p.HC + uw;
+        const int kvh = p.per_head ? (list - b * p.Hq) / p.G : unit / p.groups;
+        const int hq0 = p.per_head ? list - b * p.Hq : kvh * p.G + (unit - kvh * p.groups) * p.rows;
+        const int heads = p.per_head ? 1 : min(p.rows, (kvh + 1) * p.G - hq0);         // query heads of this unit
+        const int seq = p.seq_lens ? max(0, min(p.seq_lens[b], p.seq_len)) : p.seq_len;
+
+        // ---- Q fragments, scaled to [2^11, 2^12) per head
+        uint32_t qa[NR][KS][2], ql[QS ? NR : 1][QS ? KS : 1][2];
+        float qn[NR];                                                    // undoes the scaling and applies sm_scale
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = g + 8 * r;
+            const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)b * p.Hq + hq0 + (row < heads ? row : 0)) * D;
+            float f[KS][4], top = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                load4(qrow + (ks >> 2) * 64 + t * 16 + (ks & 3) * 4, f[ks]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = fabsf(f[ks][i]);
+                    top = a < INFINITY ? fmaxf(top, a) : top;
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int sh = 138 - (int)(__float_as_uint(top) >> 23);           // 11 less the exponent of the largest element
+            sh = top == 0.f ? 0 : min(sh, 120);
+            const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+            qn[r] = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x0 = f[ks][2 * i] * up, x1 = f[ks][2 * i + 1] * up;
+                    qa[r][ks][i] = row < heads ? pack_f16(x0, x1) : 0u;
+                    if (QS) ql[QS ? r : 0][QS ? ks : 0][i] = row < heads ? pack_f16_rest(x0, x1, qa[r][ks][i]) : 0u;
+                }
+        }
+
+        float o[NR][KS][4];
+        float m[NR], M[NR], l[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            m[r] = M[r] = -FLT_MAX;
+            l[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][j][i] = 0.f;
+        }
+
+        // ---- looking tokens up: lane i and lane 16 + i follow token i of a tile; its list entry is loaded two tiles
+        //      ahead of its copies, its page one tile ahead
+        const int tk = lane & 15;
+        const size_t pitch = (size_t)p.Hkv * D;
         const int ps = p.map.page_size;
-        float kv[2][EPL];
+        auto fetch_pos = [&](int it) -> int {
+            const int i = tok0 + (it * TG + tg) * kKv8Tile + tk;
+            if (it >= n_it || i >= tok1) return INT_MIN;                 // no token here
+            return p.sel_idx ? max(p.sel_idx[(size_t)list * p.sel_stride + i], -1) : i;
+        };
+        auto fetch_page = [&](int pos) -> int {
+            if (pos < 0 || pos >= seq) return -1;
+            const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / ps;
+            return p.map.page_table ? p.map.page_table[(size_t)b * p.map.pt_stride + pg] : (int)((int64_t)b * p.map.pt_stride + pg);
+        };
+        int pos_c = fetch_pos(0), page_c = fetch_page(pos_c), pos_n = fetch_pos(1);
+        uint32_t sc_new = 0;
+        auto issue = [&](int it) {
+            // pool row of token tk (its V row lies ps rows further), or -1
+            int row = -1;
+            sc_new = 0;
+            if (page_c >= 0 && page_c < p.map.num_pages) {
+                const int pg = p.page_shift >= 0 ? pos_c >> p.page_shift : pos_c / ps;
+                const int entry = pos_c - pg * ps;
+                row = page_c * 2 * ps + entry;
+                const int blk = p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block;
+                const int per_page = p.block_shift >= 0 ? ps >> p.block_shift : ps / p.block;
+                sc_new = p.scales[((size_t)((int64_t)page_c * 2 + (lane >> 4)) * per_page + blk) * p.Hkv + kvh] | 0x100u;
+            } else if (pos_c != INT_MIN) {
+                if (lane < 16) atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
+            }
+            unsigned char* dst = ring + (size_t)(it % S) * Kv8Ring<D>::stage_bytes;
 #pragma unroll
-        for (int pl = 0; pl < 2; ++pl) {
-            const uint8_t* c = p.kv + (((size_t)page * 2 + pl) * ps + entry) * p.Hkv * D + (size_t)h * D + lane * EPL;
-            const float sc = scale_value(p.scales[(((size_t)page * 2 + pl) * (ps / p.block) + entry / p.block) * p.Hkv + h]);
+            for (int n2 = 0; n2 < 2; ++n2) {
+                const int r = __shfl_sync(0xffffffffu, row, n2 * 8 + g);
+                const uint8_t* src = p.kv + (size_t)max(r, 0) * pitch + (size_t)kvh * D + t * 16;
 #pragma unroll
-            for (int i = 0; i < EPL; i += 2) {
-                const float2 f = unpack_e4m3(*reinterpret_cast<const uint16_t*>(c + i));
-                kv[pl][i] = f.x * sc;
-                kv[pl][i + 1] = f.y * sc;
+                for (int c = 0; c < KC; ++c) cp_async16(dst + ((n2 * KC + c) * 32 + lane) * 16, src + c * 64, r >= 0);
+            }
+            dst += kKv8Tile * D;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = __shfl_sync(0xffffffffu, row, 2 * t + (i & 1) + (i >> 1) * 8);
+                const uint8_t* src = p.kv + (size_t)(max(r, 0) + ps) * pitch + (size_t)kvh * D + g * VB;
+                if (VB == 16) cp_async16(dst + (i * 32 + lane) * 16, src, r >= 0);
+                else cp_async8(dst + (i * 32 + lane) * 8, src, r >= 0);
+            }
+            page_c = fetch_page(pos_n);
+            pos_c = pos_n;
+            pos_n = fetch_pos(it + 2);
+        };
+        auto park_scales = [&](int it) {                                 // scale bytes of tile `it`, loaded when it was issued
+            uint16_t* at = reinterpret_cast<uint16_t*>(&sc_ring[warp][it % S][tk]) + (lane >> 4);
+            *at = (uint16_t)sc_new;
+        };
+
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) {
+            if (s < n_it) {
+                issue(s);
+                park_scales(s);
+            }
+            cp_async_commit();
+        }
+        for (int it = 0; it < n_it; ++it) {
+            const bool more = it + S - 1 < n_it;
+            if (more) issue(it + S - 1);
+            cp_async_commit();
+            cp_async_wait<S - 1>();
+            __syncwarp();
+            const unsigned char* st = ring + (size_t)(it % S) * Kv8Ring<D>::stage_bytes;
+            // ---- S = Q K^T
+            float sf[2][4];
+#pragma unroll
+            for (int n2 = 0; n2 < 2; ++n2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sf[n2][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const uint4 kw = *reinterpret_cast<const uint4*>(st + ((n2 * KC + c) * 32 + lane) * 16);
+                    const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t b0, b1;
+                        halves_of(w[i], b0, b1);
+                        const int ks = c * 4 + i;
+                        mma_f16(sf[n2], qa[0][ks][0], R2 ? qa[NR - 1][ks][0] : 0u, qa[0][ks][1], R2 ? qa[NR - 1][ks][1] : 0u, b0, b1);
+                        if (QS) mma_f16(sf[n2], ql[0][QS ? ks : 0][0], R2 ? ql[QS ? NR - 1 : 0][QS ? ks : 0][0] : 0u, ql[0][QS ? ks : 0][1],
+                                        R2 ? ql[QS ? NR - 1 : 0][QS ? ks : 0][1] : 0u, b0, b1);
+                    }
+                }
+            }
+            // ---- scales of this lane's four tokens (2t, 2t+1, 8+2t, 9+2t)
+            const uint2 s01 = *reinterpret_cast<const uint2*>(&sc_ring[warp][it % S][2 * t]);
+            const uint2 s23 = *reinterpret_cast<const uint2*>(&sc_ring[warp][it % S][8 + 2 * t]);
+            const uint32_t sc[4] = {s01.x, s01.y, s23.x, s23.y};
+            const int i0 = tok0 + (it * TG + tg) * kKv8Tile + 2 * t;     // list index of the lane's first token
+            uint32_t pb[NR][2], pl[PS ? NR : 1][2];
+            float x[NR][4], ev[4];
+            bool moved = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ev[i] = (float)((int)(sc[i] >> 16 & 0xffu) - 127);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float top = -FLT_MAX, topv = -FLT_MAX;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = sf[i >> 1][2 * r + (i & 1)] * scale_value(sc[i] & 0xffu) * qn[r];
+                    if (p.scores && (sc[i] & 0x100u) && g + 8 * r < heads)
+                        p.scores[((size_t)b * p.Hq + hq0 + g + 8 * r) * p.score_stride + i0 + (i >> 1) * 8 + (i & 1)] = y;
+                    x[r][i] = (sc[i] & 0x100u) ? y * kLog2e : -INFINITY;
+                    top = fmaxf(top, x[r][i]);
+                    topv = fmaxf(topv, x[r][i] + ev[i]);
+                }
+                moved |= top > m[r] || topv > M[r];
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float top = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
+                    float topv = fmaxf(fmaxf(x[r][0] + ev[0], x[r][1] + ev[1]), fmaxf(x[r][2] + ev[2], x[r][3] + ev[3]));
+#pragma unroll
+                    for (int off = 1; off < 4; off <<= 1) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                        topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
+                    }
+                    const float mn = fmaxf(m[r], ceilf(top)), Mn = fmaxf(M[r], ceilf(topv));
+                    l[r] *= fast_exp2(m[r] - mn);
+                    const float a = fast_exp2(M[r] - Mn);
+                    m[r] = mn;
+                    M[r] = Mn;
+                    const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        o[r][j][0] *= a0;
+                        o[r][j][1] *= a1;
+                        o[r][j][2] *= a0;
+                        o[r][j][3] *= a1;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    l[r] += fast_exp2(x[r][i] - m[r]);
+                    w[i] = fast_exp2(x[r][i] + (ev[i] - M[r] + 14.f));
+                }
+                pb[r][0] = pack_f16(w[0], w[1]);
+                pb[r][1] = pack_f16(w[2], w[3]);
+                if (PS) {
+                    pl[PS ? r : 0][0] = pack_f16_rest(w[0], w[1], pb[r][0]);
+                    pl[PS ? r : 0][1] = pack_f16_rest(w[2], w[3], pb[r][1]);
+                }
+            }
+            // ---- O^T += V^T P^T
+            st += kKv8Tile * D;
+            uint32_t vw[4][VB / 4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (VB == 16) {
+                    const uint4 q4 = *reinterpret_cast<const uint4*>(st + (i * 32 + lane) * 16);
+                    vw[i][0] = q4.x, vw[i][1] = q4.y, vw[i][VB / 4 - 2] = q4.z, vw[i][VB / 4 - 1] = q4.w;
+                } else {
+                    const uint2 q2 = *reinterpret_cast<const uint2*>(st + (i * 32 + lane) * 8);
+                    vw[i][0] = q2.x, vw[i][1] = q2.y;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w) {
+                uint32_t a[2][4];                                        // [token pair][element of the word], a pair of tokens each
+#pragma unroll
+                for (int h2 = 0; h2 < 2; ++h2) {
+                    halves_of(__byte_perm(vw[2 * h2][w], vw[2 * h2 + 1][w], 0x5140), a[h2][0], a[h2][1]);
+                    halves_of(__byte_perm(vw[2 * h2][w], vw[2 * h2 + 1][w], 0x7362), a[h2][2], a[h2][3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
+                        if (PS) mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[PS ? r : 0][0], pl[PS ? r : 0][1]);
+                    }
+            }
+            __syncwarp();                                                // the scale slot may be overwritten
+            if (more) park_scales(it + S - 1);
+        }
+        cp_async_wait<0>();
+
+        // ---- warps of a unit merge through shared memory: o relative to m
+        __syncthreads();
+        float* so = reinterpret_cast<float*>(smem);                      // [warps][rows][D]
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (t == 0) {
+                ml[warp][g + 8 * r][0] = m[r];
+                ml[warp][g + 8 * r][1] = l[r];
+            }
+            const float f = fast_exp2(M[r] - 14.f - m[r]);
+            const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const int h0 = 2 * t + 8 * r;
+                float* at = so + ((size_t)warp * p.rows + h0) * D + g * VB + 2 * j;
+                if (h0 < p.rows) *reinterpret_cast<float2*>(at) = make_float2(o[r][j][0] * f0, o[r][j][2] * f0);
+                if (h0 + 1 < p.rows) *reinterpret_cast<float2*>(at + D) = make_float2(o[r][j][1] * f1, o[r][j][3] * f1);
             }
         }
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s += q[i] * kv[0][i];
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= p.sm_scale;
-        if (p.scores && lane == 0) p.scores[((size_t)b * p.Hq + hq) * p.score_stride + t] = s;
-        s *= kLog2e;
-        const float mn = fmaxf(m, s), keep = mn == -INFINITY ? 1.f : fast_exp2(m - mn), w = mn == -INFINITY ? 0.f : fast_exp2(s - mn);
-        m = mn;
-        l = l * keep + w;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) o[i] = o[i] * keep + w * kv[1][i];
-    }
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) sh_o[warp][lane * EPL + i] = o[i];
-    if (lane == 0) sh_ml[warp][0] = m, sh_ml[warp][1] = l;
-    __syncthreads();
-    const size_t part = ((size_t)b * p.Hq + hq) * p.chunks + chunk;
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
-        float M = -INFINITY, L = 0.f, acc = 0.f;
-        for (int i = 0; i < kKv8Warps; ++i) M = fmaxf(M, sh_ml[i][0]);
-        for (int i = 0; i < kKv8Warps; ++i) {
-            const float w = sh_ml[i][0] == -INFINITY ? 0.f : fast_exp2(sh_ml[i][0] - M);
-            L += w * sh_ml[i][1];
-            acc += w * sh_o[i][d];
+        __syncthreads();
+        const int unit_rows = p.HC * p.rows, vecs = unit_rows * (D / 4);
+        const size_t part0 = (size_t)slice * (p.ctas + p.lists);
+        auto put = [&](int ur, int d, float4 acc, float mx, float sum) {
+            const int u = slice * p.HC + ur / p.rows, row = ur % p.rows;
+            const int kh = p.per_head ? 0 : u / p.groups;
+            const int h = p.per_head ? list - b * p.Hq : kh * p.G + (u - kh * p.groups) * p.rows + row;
+            if (!p.per_head && h >= (kh + 1) * p.G) return;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            store4(reinterpret_cast<T*>(p.o) + ((size_t)b * p.Hq + h) * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+            if (p.lse && d == 0) p.lse[(size_t)b * p.Hq + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+        };
+        for (int i = tid; i < vecs; i += blockDim.x) {
+            const int ur = i / (D / 4), d = (i - ur * (D / 4)) * 4, uu = ur / p.rows, row = ur - uu * p.rows;
+            float mx = -FLT_MAX, sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < TG; ++k) mx = fmaxf(mx, ml[uu + k * p.HC][row][0]);
+            for (int k = 0; k < TG; ++k) {
+                const int w = uu + k * p.HC;
+                const float f = fast_exp2(ml[w][row][0] - mx);
+                const float4 v = *reinterpret_cast<const float4*>(so + ((size_t)w * p.rows + row) * D + d);
+                sum = fmaf(f, ml[w][row][1], sum);
+                acc.x = fmaf(f, v.x, acc.x);
+                acc.y = fmaf(f, v.y, acc.y);
+                acc.z = fmaf(f, v.z, acc.z);
+                acc.w = fmaf(f, v.w, acc.w);
+            }
+            if (whole) {
+                put(ur, d, acc, mx, sum);
+            } else {
+                const size_t at = (part0 + cta + list) * unit_rows + ur;
+                __stcg(reinterpret_cast<float4*>(p.part_o + at * D + d), acc);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + at * 2), make_float2(mx, sum));
+            }
         }
-        p.part_o[part * D + d] = acc;
-        if (d == 0) p.part_ml[2 * part] = M, p.part_ml[2 * part + 1] = L;
+        if (!whole) {
+            // ---- the list is shared by several CTAs: the last of them to arrive merges their parts, in order
+            const int c0 = cta_of(first_tile), parts = cta_of(first_tile + n_tiles - 1) - c0 + 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                uint32_t* cnt = p.arrivals + ((size_t)list * p.slices + slice) * 16;
+                s_last = atomicAdd(cnt, 1u) == (uint32_t)parts - 1u;
+                if (s_last) *cnt = 0u;
+                __threadfence();
+            }
+            __syncthreads();
+            if (s_last) {
+                for (int i = tid; i < vecs; i += blockDim.x) {
+                    const int ur = i / (D / 4), d = (i - ur * (D / 4)) * 4;
+                    const size_t at = (part0 + c0 + list) * unit_rows + ur;
+                    float mx = -FLT_MAX, sum = 0.f;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < parts; ++k) mx = fmaxf(mx, __ldcg(p.part_ml + (at + (size_t)k * unit_rows) * 2));
+                    for (int k = 0; k < parts; ++k) {
+                        const float2 s = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (at + (size_t)k * unit_rows) * 2));
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (at + (size_t)k * unit_rows) * D + d));
+                        const float f = fast_exp2(s.x - mx);
+                        sum = fmaf(f, s.y, sum);
+                        acc.x = fmaf(f, v.x, acc.x);
+                        acc.y = fmaf(f, v.y, acc.y);
+                        acc.z = fmaf(f, v.z, acc.z);
+                        acc.w = fmaf(f, v.w, acc.w);
+                    }
+                    put(ur, d, acc, mx, sum);
+                }
+            }
+        }
+        __syncthreads();                                                 // the ring is free for the next segment
+        tile = seg_end;
+        if (p.ragged == 2) break;
     }
 }
 
-// o = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks of a query head.
 template <typename T, int D>
-__global__ void __launch_bounds__(D) merge_kv8_kernel(const AttnKv8Params p) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const size_t row = blockIdx.x;
-    const int d = threadIdx.x;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int c = 0; c < p.chunks; ++c) M = fmaxf(M, p.part_ml[2 * (row * p.chunks + c)]);
-    for (int c = 0; c < p.chunks; ++c) {
-        const float m = p.part_ml[2 * (row * p.chunks + c)];
-        const float w = m == -INFINITY ? 0.f : fast_exp2(m - M);
-        L += w * p.part_ml[2 * (row * p.chunks + c) + 1];
-        acc += w * p.part_o[(row * p.chunks + c) * D + d];
-    }
-    reinterpret_cast<T*>(p.o)[row * D + d] = from_f32<T>(L == 0.f ? 0.f : acc / L);
-    if (p.lse && d == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) / kLog2e;
-}
-
-template <typename T, int D>
-static int launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream_t st) {
-    TIDAL_CUDA_OK(launch_pdl(attn_kv8_kernel<T, D>, dim3(p.chunks, batch * p.Hq), dim3(kKv8Warps * 32), 0, st, 1, p));
-    TIDAL_CUDA_OK(launch_pdl(merge_kv8_kernel<T, D>, dim3(batch * p.Hq), dim3(D), 0, st, 1, p));
-    count_launch(2);
-    return TIDAL_OK;
+static int launch_attn_kv8(const AttnKv8Params& p, cudaStream_t st) {
+    const size_t smem = Kv8Ring<D>::bytes + (p.ragged == 1 ? sizeof(int) * (p.lists + 1) : 0);
+    auto go = [&](auto kern) -> int {
+        TIDAL_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TIDAL_CUDA_OK(launch_pdl(kern, dim3(p.ctas, p.slices), dim3(kKv8Warps * 32), smem, st, 1, p));
+        count_launch();
+        return TIDAL_OK;
+    };
+    return p.rows > 8 ? go(attn_kv8_kernel<T, D, true>) : go(attn_kv8_kernel<T, D, false>);
 }
 
 }  // namespace tidal
@@ -169,19 +601,43 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     p.scores = a->d_scores; p.score_stride = a->score_stride; p.lse = a->d_lse;
     p.part_o = (float*)((char*)d_ws + L->part_o_off);
     p.part_ml = (float*)((char*)d_ws + L->part_ml_off);
+    p.arrivals = (uint32_t*)((char*)d_ws + L->xc_off);
     p.status = (uint32_t*)((char*)d_ws + L->status_off);
     p.Hq = a->num_qo_heads; p.Hkv = a->num_kv_heads; p.G = a->num_qo_heads / a->num_kv_heads; p.block = a->block;
-    p.chunks = tidal_plan_chunks(a->batch, a->num_qo_heads, ntok, 64, 4 * sm_count_cached());
     p.sm_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / sqrtf((float)a->head_dim);
-    TIDAL_REQUIRE((int64_t)a->batch * a->num_qo_heads <= 65535, TIDAL_ERR_ARG, "batch * num_qo_heads beyond 65535");
-    const size_t rows = (size_t)a->batch * a->num_qo_heads * p.chunks;
-    TIDAL_REQUIRE(L->part_o_off + sizeof(float) * rows * a->head_dim <= L->part_ml_off && L->part_ml_off + sizeof(float) * rows * 2 <= L->hist_off,
+    auto shift_of = [](int x) { return (x & (x - 1)) == 0 ? 31 - __builtin_clz((unsigned)x) : -1; };
+    p.page_shift = shift_of(a->page_size);
+    p.block_shift = shift_of(a->block);
+    p.per_head = p.sel_rows != 1;
+    const int64_t lists = (int64_t)a->batch * p.sel_rows;
+    TIDAL_REQUIRE(lists <= 1 << 20, TIDAL_ERR_ARG, "attention_kv8: more than 2^20 token lists");
+    p.lists = (int)lists;
+    const int G = p.per_head ? 1 : p.G;
+    p.groups = (G + 15) / 16;
+    p.rows = (G + p.groups - 1) / p.groups;
+    const int units = p.per_head ? 1 : p.Hkv * p.groups;
+    p.HC = 1;
+    p.slices = units / p.HC;
+    const int TT = kKv8Tile * (kKv8Warps / p.HC);
+    const bool ragged = sel ? p.sel_counts != nullptr : p.seq_lens != nullptr;
+    p.ragged = !ragged ? 0 : p.lists <= kKv8MaxPrefix ? 1 : 2;
+    p.tiles_per_list = ntok > 0 ? (ntok + TT - 1) / TT : 1;
+    const int64_t most_tiles = (int64_t)p.tiles_per_list * p.lists;
+    TIDAL_REQUIRE(most_tiles <= INT32_MAX, TIDAL_ERR_ARG, "attention_kv8: more than 2^31 tiles of tokens");
+    // two CTAs to an SM share the tiles, at least two tiles each
+    int64_t ctas = 2 * sm_count_cached() / p.slices;
+    ctas = std::max<int64_t>(1, std::min<int64_t>(ctas, (most_tiles + 1) / 2));
+    p.ctas = p.ragged == 2 ? p.lists : (int)ctas;
+    TIDAL_REQUIRE(p.slices <= 65535, TIDAL_ERR_ARG, "attention_kv8: more than 65535 head slices");
+    const size_t parts = (size_t)p.slices * (p.ctas + p.lists) * p.HC * p.rows;
+    TIDAL_REQUIRE(p.ragged == 2 || (L->part_o_off + sizeof(float) * parts * a->head_dim <= L->part_ml_off && L->part_ml_off + sizeof(float) * parts * 2 <= L->hist_off &&
+                                    L->xc_off + sizeof(uint32_t) * 16 * (size_t)p.lists * p.slices <= L->cand_off),
                   TIDAL_ERR_WORKSPACE, "workspace was sized for a smaller batch/heads/head_dim than this call");
     cudaStream_t st = (cudaStream_t)stream;
     const bool wide = a->head_dim == 128;
     switch (a->dtype) {
-        case TIDAL_DTYPE_F16: return wide ? launch_attn_kv8<__half, 128>(p, a->batch, st) : launch_attn_kv8<__half, 64>(p, a->batch, st);
-        case TIDAL_DTYPE_BF16: return wide ? launch_attn_kv8<__nv_bfloat16, 128>(p, a->batch, st) : launch_attn_kv8<__nv_bfloat16, 64>(p, a->batch, st);
-        default: return wide ? launch_attn_kv8<float, 128>(p, a->batch, st) : launch_attn_kv8<float, 64>(p, a->batch, st);
+        case TIDAL_DTYPE_F16: return wide ? launch_attn_kv8<__half, 128>(p, st) : launch_attn_kv8<__half, 64>(p, st);
+        case TIDAL_DTYPE_BF16: return wide ? launch_attn_kv8<__nv_bfloat16, 128>(p, st) : launch_attn_kv8<__nv_bfloat16, 64>(p, st);
+        default: return wide ? launch_attn_kv8<float, 128>(p, st) : launch_attn_kv8<float, 64>(p, st);
     }
 }
