@@ -15,13 +15,15 @@
 // step is 2^-12, next to 2^-9 for a bf16 result; for fp16 and fp32 results a second fp16 term carries the remainder.
 // Accumulators, maxima and sums are fp32.
 //
-// Data movement.  The order of the contraction index and of the output elements is free as long as both operands agree, so
-// every lane copies exactly the bytes that its own fragments need (cp.async, 16 bytes at a time) into a ring of
-// shared memory that no other lane reads: no barrier, no bank conflict, no register held by data in flight.  With
-// lane = 4 g + t, a tile of 16 tokens:
-//     S = Q K^T  (M = heads, N = tokens): lane holds 64-byte pieces t*16.. of K rows g and 8+g; the four bytes of one
+// Data movement.  Every warp has a ring of tiles of its own in shared memory, filled with cp.async, 16 bytes to a lane and a
+// whole row to adjacent lanes (with the two pieces of a 32-byte sector four lanes apart, sectors were fetched twice: 6.0
+// TB/s left L2 for 4.0 TB/s of cache).  No barrier beyond the warp's own, no register held by data in flight.  The order of
+// the contraction index and of the output elements is free as long as both operands agree, so the fragments are read
+// 16 bytes at a time, from 16-byte pieces that are permuted within 128 bytes so that no two lanes of an access meet
+// in a bank.  With lane = 4 g + t, a tile of 16 tokens:
+//     S = Q K^T  (M = heads, N = tokens): lane reads 16-byte pieces t, 4 + t of K rows g and 8+g; the four bytes of one
 //                word are elements 2t, 2t+1, 2t+8, 2t+9 of a k-step
-//     O^T = V^T P^T  (M = elements, N = heads): lane holds bytes g*D/8.. of V rows 2t, 2t+1, 2t+8, 2t+9, and the
+//     O^T = V^T P^T  (M = elements, N = heads): lane reads bytes g*D/8.. of V rows 2t, 2t+1, 2t+8, 2t+9, and the
 //                accumulator of S already has the layout of the B operand P^T
 #include <algorithm>
 #include <cfloat>
@@ -33,7 +35,7 @@
 namespace tidal {
 
 constexpr int kKv8Warps = 8;
-constexpr int kKv8Tile = 16;             // tokens a warp takes at a time
+constexpr int kKv8Tile = 16;             // tokens a warp takes at a time; it looks them up two tiles at a time
 constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself
 
 struct AttnKv8Params {
@@ -68,9 +70,6 @@ struct AttnKv8Params {
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async8(void* dst, const void* src, bool valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 8 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -107,6 +106,16 @@ struct Kv8Ring {
     static constexpr int stage_bytes = kKv8Tile * 2 * D;                 // of one warp: K rows, then V rows
     static constexpr size_t bytes = (size_t)kKv8Warps * stages * stage_bytes;
 };
+// Byte offset of 16-byte piece c of token i's K row / V row within a tile.  Eight lanes of an access (a quarter of a warp,
+// or half of one where a lane reads 8 bytes) have to fall into the eight different pieces of 128 bytes: K rows are
+// read by two neighbouring tokens and four neighbouring pieces, V rows by four tokens of one parity and 32 bytes.
+template <int D>
+__device__ __forceinline__ int k_piece(int i, int c) { return D == 128 ? i * 128 + (c ^ (i & 1) * 4) * 16 : i * 64 + c * 16; }
+template <int D>
+__device__ __forceinline__ int v_piece(int i, int c) {
+    if (D == 128) return i * 128 + (c ^ (i & 6)) * 16;
+    return (i >> 1) * 128 + ((i ^ i >> 1) & 1) * 64 + (c ^ (i >> 1 & 2)) * 16;
+}
 // Four consecutive elements of a row.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float* f) {
@@ -135,14 +144,16 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
     constexpr bool QS = sizeof(T) == 4, PS = !std::is_same<T, __nv_bfloat16>::value;
     constexpr int S = Kv8Ring<D>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t sc_ring[kKv8Warps][S][kKv8Tile];                 // per token: K scale byte, valid, V scale byte
+    constexpr int NP = S <= 4 ? 2 : 4;       // pairs of tiles whose scales are kept: a slot is refilled S - 2 NP <= 0 tiles after its last use
+    // per token: scale of K (-1: no token) and exponent of the scale of V (-inf: the block reads as zeros)
+    __shared__ __align__(16) float2 sc_ring[kKv8Warps][NP][2 * kKv8Tile];
     __shared__ float ml[kKv8Warps][16][2];
     __shared__ int s_scan[kKv8Warps + 1];
     __shared__ int s_last;
     int* prefix = reinterpret_cast<int*>(smem + Kv8Ring<D>::bytes);    // [lists + 1] when the lengths are added up here
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int TG = kKv8Warps / p.HC, TT = kKv8Tile * TG;
+    const int TG = kKv8Warps / p.HC, TT = 2 * kKv8Tile * TG;
     const int uw = warp % p.HC, tg = warp / p.HC;
     const int cta = blockIdx.x, slice = blockIdx.y;
     unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D>::stage_bytes;
@@ -210,7 +221,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
         const bool whole = p.ragged == 2 || (tile == first_tile && seg_end == first_tile + n_tiles);
         const int tok0 = p.ragged == 2 ? 0 : (int)min((int64_t)len, (tile - first_tile) * TT);
         const int tok1 = p.ragged == 2 ? len : (int)min((int64_t)len, (int64_t)(seg_end - first_tile) * TT);
-        const int n_it = (tok1 - tok0 + TT - 1) / TT;
+        const int w0 = tok0 + tg * 2 * kKv8Tile;                         // first token of this warp; it takes 32 of every TT
+        const int n_pairs = tok1 > w0 ? (tok1 - w0 + TT - 1) / TT : 0;
+        int n_it = 2 * n_pairs;                                          // its tiles (an empty one at the end is left out)
+        if (n_pairs > 0 && w0 + (n_pairs - 1) * TT + kKv8Tile >= tok1) --n_it;
 
         const int b = p.per_head ? list / p.Hq : list;
         const int unit = slice * p.HC + uw;
@@ -221,7 +235,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
 
         // ---- Q fragments, scaled to [2^11, 2^12) per head
         uint32_t qa[NR][KS][2], ql[QS ? NR : 1][QS ? KS : 1][2];
-        float qn[NR];                                                    // undoes the scaling and applies sm_scale
+        float qn[NR], qn2[NR];                                           // undo the scaling and apply sm_scale (in log2 units)
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const int row = g + 8 * r;
@@ -242,6 +256,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             sh = top == 0.f ? 0 : min(sh, 120);
             const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
             qn[r] = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+            qn2[r] = qn[r] * kLog2e;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -264,14 +279,19 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                 for (int i = 0; i < 4; ++i) o[r][j][i] = 0.f;
         }
 
-        // ---- looking tokens up: lane i and lane 16 + i follow token i of a tile; its list entry is loaded two tiles
-        //      ahead of its copies, its page one tile ahead
-        const int tk = lane & 15;
+        // ---- looking tokens up: lane i follows token i of a pair of tiles; its list entry is loaded two pairs ahead of
+        //      its copies, its page one pair ahead, its scales with the copies
         const size_t pitch = (size_t)p.Hkv * D;
         const int ps = p.map.page_size;
-        auto fetch_pos = [&](int it) -> int {
-            const int i = tok0 + (it * TG + tg) * kKv8Tile + tk;
-            if (it >= n_it || i >= tok1) return INT_MIN;                 // no token here
+        constexpr int PR = D / 16, TI = 32 / PR;                          // 16-byte pieces of a row; tokens that one copy of the warp covers
+        const int c_tok = lane / PR, c_piece = lane % PR;
+        const uint8_t* k_src = p.kv + (size_t)kvh * D + c_piece * 16;
+        const size_t v_plane = (size_t)ps * pitch;
+        const int k_off = k_piece<D>(g, t), v_off = v_piece<D>(2 * t, g * VB / 16) + (g * VB & 15);
+        const int v_off1 = v_piece<D>(2 * t + 1, g * VB / 16) + (g * VB & 15);
+        auto fetch_pos = [&](int pair) -> int {
+            const int i = w0 + pair * TT + lane;
+            if (pair >= n_pairs || i >= tok1) return INT_MIN;            // no token here
             return p.sel_idx ? max(p.sel_idx[(size_t)list * p.sel_stride + i], -1) : i;
         };
         auto fetch_page = [&](int pos) -> int {
@@ -280,61 +300,67 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             return p.map.page_table ? p.map.page_table[(size_t)b * p.map.pt_stride + pg] : (int)((int64_t)b * p.map.pt_stride + pg);
         };
         int pos_c = fetch_pos(0), page_c = fetch_page(pos_c), pos_n = fetch_pos(1);
-        uint32_t sc_new = 0;
-        auto issue = [&](int it) {
-            // pool row of token tk (its V row lies ps rows further), or -1
-            int row = -1;
-            sc_new = 0;
+        int row = -1;                                                    // pool row of the lane's K row (its V row lies ps rows further), or -1
+        uint32_t sc_k = 0, sc_v = 0;                                     // its scale bytes
+        uint32_t full = 0;                                               // bit i: every token of the pair issued i pairs ago is there
+        auto look_up = [&](int pair) {
+            row = -1;
             if (page_c >= 0 && page_c < p.map.num_pages) {
                 const int pg = p.page_shift >= 0 ? pos_c >> p.page_shift : pos_c / ps;
                 const int entry = pos_c - pg * ps;
                 row = page_c * 2 * ps + entry;
                 const int blk = p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block;
                 const int per_page = p.block_shift >= 0 ? ps >> p.block_shift : ps / p.block;
-                sc_new = p.scales[((size_t)((int64_t)page_c * 2 + (lane >> 4)) * per_page + blk) * p.Hkv + kvh] | 0x100u;
+                const uint8_t* at = p.scales + ((size_t)page_c * 2 * per_page + blk) * p.Hkv + kvh;
+                sc_k = at[0];
+                sc_v = at[(size_t)per_page * p.Hkv];
             } else if (pos_c != INT_MIN) {
-                if (lane < 16) atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
+                atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
             }
-            unsigned char* dst = ring + (size_t)(it % S) * Kv8Ring<D>::stage_bytes;
-#pragma unroll
-            for (int n2 = 0; n2 < 2; ++n2) {
-                const int r = __shfl_sync(0xffffffffu, row, n2 * 8 + g);
-                const uint8_t* src = p.kv + (size_t)max(r, 0) * pitch + (size_t)kvh * D + t * 16;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) cp_async16(dst + ((n2 * KC + c) * 32 + lane) * 16, src + c * 64, r >= 0);
-            }
-            dst += kKv8Tile * D;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = __shfl_sync(0xffffffffu, row, 2 * t + (i & 1) + (i >> 1) * 8);
-                const uint8_t* src = p.kv + (size_t)(max(r, 0) + ps) * pitch + (size_t)kvh * D + g * VB;
-                if (VB == 16) cp_async16(dst + (i * 32 + lane) * 16, src, r >= 0);
-                else cp_async8(dst + (i * 32 + lane) * 8, src, r >= 0);
-            }
+            full = full << 1 | (__all_sync(0xffffffffu, row >= 0) ? 1u : 0u);
             page_c = fetch_page(pos_n);
             pos_c = pos_n;
-            pos_n = fetch_pos(it + 2);
+            pos_n = fetch_pos(pair + 2);
         };
-        auto park_scales = [&](int it) {                                 // scale bytes of tile `it`, loaded when it was issued
-            uint16_t* at = reinterpret_cast<uint16_t*>(&sc_ring[warp][it % S][tk]) + (lane >> 4);
-            *at = (uint16_t)sc_new;
+        auto park_scales = [&](int pair) {
+            sc_ring[warp][pair & (NP - 1)][lane] = row >= 0 ? make_float2(scale_value(sc_k), sc_v ? (float)((int)sc_v - 127) : -INFINITY) : make_float2(-1.f, -INFINITY);
+        };
+        auto copy = [&](int it, unsigned char* dst) {
+            const int l0 = (it & 1) * kKv8Tile + c_tok;
+            const bool all = full & 1u;
+#pragma unroll
+            for (int i = 0; i < kKv8Tile / TI; ++i) {
+                const int r = __shfl_sync(0xffffffffu, row, l0 + i * TI);
+                const uint8_t* src = k_src + (all ? (uint32_t)r : (uint32_t)max(r, 0)) * pitch;
+                cp_async16(dst + k_piece<D>(i * TI + c_tok, c_piece), src, all || r >= 0);
+                cp_async16(dst + kKv8Tile * D + v_piece<D>(i * TI + c_tok, c_piece), src + v_plane, all || r >= 0);
+            }
         };
 
+        int put_slot = 0, use_slot = 0;
 #pragma unroll
         for (int s = 0; s < S - 1; ++s) {
             if (s < n_it) {
-                issue(s);
-                park_scales(s);
+                if ((s & 1) == 0) {
+                    look_up(s >> 1);
+                    park_scales(s >> 1);
+                }
+                copy(s, ring + s * Kv8Ring<D>::stage_bytes);
             }
             cp_async_commit();
         }
+        put_slot = S - 1;
         for (int it = 0; it < n_it; ++it) {
-            const bool more = it + S - 1 < n_it;
-            if (more) issue(it + S - 1);
+            const int ahead = it + S - 1;
+            const bool looked = ahead < n_it && (ahead & 1) == 0;
+            if (looked) look_up(ahead >> 1);
+            if (ahead < n_it) copy(ahead, ring + put_slot * Kv8Ring<D>::stage_bytes);
+            put_slot = put_slot == S - 1 ? 0 : put_slot + 1;
             cp_async_commit();
             cp_async_wait<S - 1>();
             __syncwarp();
-            const unsigned char* st = ring + (size_t)(it % S) * Kv8Ring<D>::stage_bytes;
+            const unsigned char* st = ring + use_slot * Kv8Ring<D>::stage_bytes;
+            use_slot = use_slot == S - 1 ? 0 : use_slot + 1;
             // ---- S = Q K^T
             float sf[2][4];
 #pragma unroll
@@ -343,7 +369,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                 for (int i = 0; i < 4; ++i) sf[n2][i] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
-                    const uint4 kw = *reinterpret_cast<const uint4*>(st + ((n2 * KC + c) * 32 + lane) * 16);
+                    const uint4 kw = *reinterpret_cast<const uint4*>(st + n2 * 8 * D + (k_off ^ c * 64));
                     const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -357,40 +383,59 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                 }
             }
             // ---- scales of this lane's four tokens (2t, 2t+1, 8+2t, 9+2t)
-            const uint2 s01 = *reinterpret_cast<const uint2*>(&sc_ring[warp][it % S][2 * t]);
-            const uint2 s23 = *reinterpret_cast<const uint2*>(&sc_ring[warp][it % S][8 + 2 * t]);
-            const uint32_t sc[4] = {s01.x, s01.y, s23.x, s23.y};
-            const int i0 = tok0 + (it * TG + tg) * kKv8Tile + 2 * t;     // list index of the lane's first token
-            uint32_t pb[NR][2], pl[PS ? NR : 1][2];
-            float x[NR][4], ev[4];
-            bool moved = false;
+            const float2* scp = &sc_ring[warp][(it >> 1) & (NP - 1)][(it & 1) * kKv8Tile + 2 * t];
+            const float4 s01 = *reinterpret_cast<const float4*>(scp), s23 = *reinterpret_cast<const float4*>(scp + 8);
+            const float kf[4] = {s01.x, s01.z, s23.x, s23.z}, ev[4] = {s01.y, s01.w, s23.y, s23.w};
+            // the pair of tile `it` was looked up ((ahead or the last tile) / 2 - it / 2) pairs before the newest one
+            const bool all = full >> ((min(ahead, n_it - 1) >> 1) - (it >> 1)) & 1u;
+            if (p.scores) {
+                const int i0 = w0 + (it >> 1) * TT + (it & 1) * kKv8Tile + 2 * t;      // list index of the lane's first token
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ev[i] = (float)((int)(sc[i] >> 16 & 0xffu) - 127);
+                for (int r = 0; r < NR; ++r)
+                    if (g + 8 * r < heads) {
+                        float* at = p.scores + ((size_t)b * p.Hq + hq0 + g + 8 * r) * p.score_stride + i0;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                float top = -FLT_MAX, topv = -FLT_MAX;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float y = sf[i >> 1][2 * r + (i & 1)] * scale_value(sc[i] & 0xffu) * qn[r];
-                    if (p.scores && (sc[i] & 0x100u) && g + 8 * r < heads)
-                        p.scores[((size_t)b * p.Hq + hq0 + g + 8 * r) * p.score_stride + i0 + (i >> 1) * 8 + (i & 1)] = y;
-                    x[r][i] = (sc[i] & 0x100u) ? y * kLog2e : -INFINITY;
-                    top = fmaxf(top, x[r][i]);
-                    topv = fmaxf(topv, x[r][i] + ev[i]);
-                }
-                moved |= top > m[r] || topv > M[r];
+                        for (int i = 0; i < 4; ++i)
+                            if (kf[i] >= 0.f) at[(i >> 1) * 8 + (i & 1)] = sf[i >> 1][2 * r + (i & 1)] * kf[i] * qn[r];
+                    }
             }
-            if (__any_sync(0xffffffffu, moved)) {
+            // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M + 14 for the weights
+            uint32_t pb[NR][2], pl[PS ? NR : 1][2];
+            float xl[NR][4], xw[NR][4];
+            auto exponents = [&]() -> bool {
+                bool moved = false;
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    float top = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
-                    float topv = fmaxf(fmaxf(x[r][0] + ev[0], x[r][1] + ev[1]), fmaxf(x[r][2] + ev[2], x[r][3] + ev[3]));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = kf[i] * qn2[r], y = sf[i >> 1][2 * r + (i & 1)];
+                        xl[r][i] = fmaf(y, f, -m[r]);
+                        xw[r][i] = fmaf(y, f, ev[i] - M[r]);
+                        if (!all && kf[i] < 0.f) xl[r][i] = -INFINITY;
+                    }
+                    moved |= fmaxf(fmaxf(xl[r][0], xl[r][1]), fmaxf(xl[r][2], xl[r][3])) > 0.f ||
+                             fmaxf(fmaxf(xw[r][0], xw[r][1]), fmaxf(xw[r][2], xw[r][3])) > 14.f;
+                }
+                return moved;
+            };
+            if (__any_sync(0xffffffffu, exponents())) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float top = -FLT_MAX, topv = -FLT_MAX;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (kf[i] >= 0.f) {
+                            const float x = sf[i >> 1][2 * r + (i & 1)] * (kf[i] * qn2[r]);
+                            top = fmaxf(top, x);
+                            topv = fmaxf(topv, x + ev[i]);
+                        }
 #pragma unroll
                     for (int off = 1; off < 4; off <<= 1) {
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
                         topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
                     }
-                    const float mn = fmaxf(m[r], ceilf(top)), Mn = fmaxf(M[r], ceilf(topv));
+                    // M is kept less the 14 of the weights' range
+                    const float mn = fmaxf(m[r], ceilf(top)), Mn = fmaxf(M[r], ceilf(topv) - 14.f);
                     l[r] *= fast_exp2(m[r] - mn);
                     const float a = fast_exp2(M[r] - Mn);
                     m[r] = mn;
@@ -404,15 +449,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                         o[r][j][3] *= a1;
                     }
                 }
+                exponents();
             }
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 float w[4];
+                l[r] += (fast_exp2(xl[r][0]) + fast_exp2(xl[r][1])) + (fast_exp2(xl[r][2]) + fast_exp2(xl[r][3]));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    l[r] += fast_exp2(x[r][i] - m[r]);
-                    w[i] = fast_exp2(x[r][i] + (ev[i] - M[r] + 14.f));
-                }
+                for (int i = 0; i < 4; ++i) w[i] = fast_exp2(xw[r][i]);
                 pb[r][0] = pack_f16(w[0], w[1]);
                 pb[r][1] = pack_f16(w[2], w[3]);
                 if (PS) {
@@ -426,10 +470,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (VB == 16) {
-                    const uint4 q4 = *reinterpret_cast<const uint4*>(st + (i * 32 + lane) * 16);
+                    const uint4 q4 = *reinterpret_cast<const uint4*>(st + (i >> 1) * 8 * D + (i & 1 ? v_off1 : v_off));
                     vw[i][0] = q4.x, vw[i][1] = q4.y, vw[i][VB / 4 - 2] = q4.z, vw[i][VB / 4 - 1] = q4.w;
                 } else {
-                    const uint2 q2 = *reinterpret_cast<const uint2*>(st + (i * 32 + lane) * 8);
+                    const uint2 q2 = *reinterpret_cast<const uint2*>(st + (i >> 1) * 8 * D + (i & 1 ? v_off1 : v_off));
                     vw[i][0] = q2.x, vw[i][1] = q2.y;
                 }
             }
@@ -449,8 +493,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                         if (PS) mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[PS ? r : 0][0], pl[PS ? r : 0][1]);
                     }
             }
-            __syncwarp();                                                // the scale slot may be overwritten
-            if (more) park_scales(it + S - 1);
+            if (looked) park_scales(ahead >> 1);
+            __syncwarp();                                                // the tile's slot is the next to be filled
         }
         cp_async_wait<0>();
 
@@ -465,7 +509,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                 ml[warp][g + 8 * r][0] = m[r];
                 ml[warp][g + 8 * r][1] = l[r];
             }
-            const float f = fast_exp2(M[r] - 14.f - m[r]);
+            const float f = fast_exp2(M[r] - m[r]);
             const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
@@ -618,7 +662,7 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     const int units = p.per_head ? 1 : p.Hkv * p.groups;
     p.HC = 1;
     p.slices = units / p.HC;
-    const int TT = kKv8Tile * (kKv8Warps / p.HC);
+    const int TT = 2 * kKv8Tile * (kKv8Warps / p.HC);
     const bool ragged = sel ? p.sel_counts != nullptr : p.seq_lens != nullptr;
     p.ragged = !ragged ? 0 : p.lists <= kKv8MaxPrefix ? 1 : 2;
     p.tiles_per_list = ntok > 0 ? (ntok + TT - 1) / TT : 1;

@@ -463,38 +463,60 @@ def qkv_rope_append(x: torch.Tensor, weight: torch.Tensor, q_out: torch.Tensor, 
 
 
 # ------------------------------------------------------------------ 8-bit KV cache
-def _launch(fn, what: str, device: torch.device, *args) -> None:
-    """fn(*args, stream) on the tensors' device and its current stream."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+def _launch(fn, what: str, index: int, *args) -> None:
+    """fn(*args, stream) on device `index` and its current stream.  Decode steps make this call per operator and layer:
+    the stream handle is taken without building a Stream object (3 us)."""
+    if index == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _stream()), what)
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
-def _need_on(device: torch.device, *ts):
-    _need_cuda(*ts)
+def _need_on(index: int, *ts) -> None:
+    """Every given tensor is contiguous and on device `index`."""
     for t in ts:
-        if t is not None and t.device != device:
-            raise RuntimeError(f"tensors must be on one device ({device} and {t.device})")
+        if t is not None:
+            if t.get_device() != index or index < 0:
+                raise RuntimeError("tensors must be CUDA tensors of one device (there is no CPU path)")
+            if not t.is_contiguous():
+                raise RuntimeError("tensors must be contiguous")
 
 
-def _need_i32(name: str, t: Optional[torch.Tensor], *shape):
-    """t is None or an int32 tensor of this shape (None: any extent)."""
-    if t is not None and (t.dtype != torch.int32 or t.dim() != len(shape) or any(w is not None and s != w for s, w in zip(t.shape, shape))):
-        raise RuntimeError(f"{name} must be int32 {['any' if w is None else w for w in shape]}, got {t.dtype} {list(t.shape)}")
+def _need_rows(name: str, t: Optional[torch.Tensor], rows: int, dtype: torch.dtype = torch.int32) -> int:
+    """t is None (0) or a [rows, n] tensor of this type: n."""
+    if t is None:
+        return 0
+    shape = t.shape
+    if t.dtype != dtype or len(shape) != 2 or shape[0] != rows:
+        raise RuntimeError(f"{name} must be {dtype} [{rows}, n], got {t.dtype} {list(shape)}")
+    return shape[1]
+
+
+def _need_vector(name: str, t: Optional[torch.Tensor], n: int) -> None:
+    """t is None or an int32 tensor of n elements."""
+    if t is not None and (t.dtype != torch.int32 or t.numel() != n):
+        raise RuntimeError(f"{name} must be int32 with {n} elements, got {t.dtype} {list(t.shape)}")
 
 
 def _kv8_geometry(kv: torch.Tensor, scales: torch.Tensor):
     """(pages, page_size, Hkv, D, block) of an 8-bit pool and its scales."""
-    if kv.dtype != torch.float8_e4m3fn or kv.dim() != 5 or kv.shape[1] != 2:
+    shape, per = kv.shape, scales.shape
+    if kv.dtype != torch.float8_e4m3fn or len(shape) != 5 or shape[1] != 2:
         raise RuntimeError("kv must be a float8_e4m3fn pool [pages,2,page_size,Hkv,D]")
-    pages, _, page_size, heads, dim = kv.shape
-    if scales.dtype != torch.uint8 or scales.dim() != 4 or scales.shape[0] != pages or scales.shape[1] != 2 or scales.shape[3] != heads:
+    pages, _, page_size, heads, dim = shape
+    if scales.dtype != torch.uint8 or len(per) != 4 or per[0] != pages or per[1] != 2 or per[3] != heads:
         raise RuntimeError("scales must be uint8 [pages,2,page_size/block,Hkv] of the same pool")
-    if scales.shape[2] < 1 or page_size % scales.shape[2]:
-        raise RuntimeError(f"scales per page ({scales.shape[2]}) must divide page_size ({page_size})")
-    return pages, page_size, heads, dim, page_size // scales.shape[2]
+    if per[2] < 1 or page_size % per[2]:
+        raise RuntimeError(f"scales per page ({per[2]}) must divide page_size ({page_size})")
+    return pages, page_size, heads, dim, page_size // per[2]
+
+
+def _kv8_pages(page_table: Optional[torch.Tensor], pages_per_seq: Optional[int], pages: int, batch: int):
+    """(address, row length) of the page table; without one, sequence b starts at page b * the row length."""
+    if page_table is not None:
+        return page_table.data_ptr(), _need_rows("page_table", page_table, batch)
+    return None, pages_per_seq if pages_per_seq is not None else pages // max(batch, 1)
 
 
 def alloc_kv8(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, block: int = 1, device="cuda") -> tuple:
@@ -521,34 +543,26 @@ def append_kv8(
 ) -> None:
     """Quantise the K,V of new tokens into an 8-bit pool; see tidal_append_kv8 in include/tidal_b200.h.  Keys are
     rotated beforehand (rope_append with kv=None)."""
-    dev = kv.device
+    dev = kv.get_device()
     _need_on(dev, kv, scales, pos0_dev, page_table, status)
     pages, page_size, heads, dim, block = _kv8_geometry(kv, scales)
+    n = k.shape[0]
     for t in (k, v):
-        if not t.is_cuda or t.device != dev:
-            raise RuntimeError("k and v must be on the pool's device")
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.dtype != k.dtype or t.shape[0] != k.shape[0]:
+        if t.get_device() != dev:
+            raise RuntimeError("k and v must be CUDA tensors of the pool's device")
+        if t.shape != (n, heads, dim) or t.dtype != k.dtype:
             raise RuntimeError(f"k and v must be [n_tokens, {heads}, {dim}] of one dtype")
-        if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        if not t.is_contiguous() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim)):
             raise RuntimeError("the heads of a token must be contiguous in k and v")
-    if batch < 1 or k.shape[0] % batch:
+    if batch < 1 or n % batch:
         raise RuntimeError("n_tokens must be a multiple of batch")
-    if k.shape[0] == 0:
+    if n == 0:
         return
-    _need_i32("pos0_dev", pos0_dev, batch)
-    _need_i32("page_table", page_table, batch, None)
-    a = _lib.AppendKv8Args()
-    a.d_k, a.d_v, a.k_stride, a.v_stride = k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0)
-    a.d_kv, a.d_scales = kv.data_ptr(), scales.data_ptr()
-    if page_table is not None:
-        a.d_page_table, a.page_table_stride = page_table.data_ptr(), page_table.shape[1]
-    else:
-        a.page_table_stride = pages_per_seq if pages_per_seq is not None else pages // batch
-    a.d_pos0, a.pos0 = _ptr(pos0_dev), int(pos0)
-    a.batch, a.tokens_per_seq, a.num_kv_heads, a.head_dim = batch, k.shape[0] // batch, heads, dim
-    a.page_size, a.block, a.dtype, a.num_pages = page_size, block, _dtype_code(k), pages
-    a.d_status = _ptr(status)
-    _launch(lib.tidal_append_kv8, "tidal_append_kv8", dev, C.byref(a))
+    _need_vector("pos0_dev", pos0_dev, batch)
+    table, row = _kv8_pages(page_table, pages_per_seq, pages, batch)
+    a = _lib.AppendKv8Args(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), kv.data_ptr(), scales.data_ptr(), table, row,
+                           _ptr(pos0_dev), pos0, batch, n // batch, heads, dim, page_size, block, _dtype_code(k), pages, _ptr(status))
+    _launch(lib.tidal_append_kv8, "tidal_append_kv8", dev, a)
 
 
 def read_kv8(kv: torch.Tensor, scales: torch.Tensor, stop: int, *, start: int = 0, batch: int = 1, dtype: torch.dtype = torch.bfloat16,
@@ -556,30 +570,23 @@ def read_kv8(kv: torch.Tensor, scales: torch.Tensor, stop: int, *, start: int = 
              out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Slots [start, stop) of every sequence of an 8-bit pool as [batch, stop - start, 2, 1, Hkv, D] rows of `dtype` (or
     of `out`): out[b] is a pool of page_size 1, as `prefill` reads it.  See tidal_read_kv8 in include/tidal_b200.h."""
-    dev = kv.device
+    dev = kv.get_device()
     _need_on(dev, kv, scales, page_table, seq_lens, out, status)
     pages, page_size, heads, dim, block = _kv8_geometry(kv, scales)
-    _need_i32("page_table", page_table, batch, None)
-    _need_i32("seq_lens", seq_lens, batch)
+    _need_vector("seq_lens", seq_lens, batch)
     if batch < 1 or start < 0 or stop < start:
         raise RuntimeError(f"bad range [{start}, {stop}) or batch {batch}")
     shape = (batch, stop - start, 2, 1, heads, dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
-    elif tuple(out.shape) != shape:
+        out = torch.empty(shape, dtype=dtype, device=kv.device)
+    elif out.shape != shape:
         raise RuntimeError(f"out must be {list(shape)}")
     if stop == start:
         return out
-    a = _lib.ReadKv8Args()
-    a.d_kv, a.d_scales, a.d_out, a.d_seq_lens = kv.data_ptr(), scales.data_ptr(), out.data_ptr(), _ptr(seq_lens)
-    if page_table is not None:
-        a.d_page_table, a.page_table_stride = page_table.data_ptr(), page_table.shape[1]
-    else:
-        a.page_table_stride = pages_per_seq if pages_per_seq is not None else pages // batch
-    a.start, a.stop, a.batch, a.num_kv_heads, a.head_dim = start, stop, batch, heads, dim
-    a.page_size, a.block, a.dtype, a.num_pages = page_size, block, _dtype_code(out), pages
-    a.d_status = _ptr(status)
-    _launch(lib.tidal_read_kv8, "tidal_read_kv8", dev, C.byref(a))
+    table, row = _kv8_pages(page_table, pages_per_seq, pages, batch)
+    a = _lib.ReadKv8Args(kv.data_ptr(), scales.data_ptr(), table, row, _ptr(seq_lens), out.data_ptr(), start, stop, batch, heads, dim,
+                         page_size, block, _dtype_code(out), pages, _ptr(status))
+    _launch(lib.tidal_read_kv8, "tidal_read_kv8", dev, a)
     return out
 
 
@@ -602,49 +609,39 @@ def decode_attention_kv8(
 ) -> torch.Tensor:
     """One decode step of attention over an 8-bit pool, all tokens or listed ones; see tidal_decode_attention_kv8 in
     include/tidal_b200.h.  `topk` ranks the logits, `accumulate_weights` takes them with the lse."""
-    dev = q.device
-    _need_on(dev, q, kv, scales, out, page_table, seq_lens, sel_idx, sel_counts, scores, lse)
+    dev = q.get_device()
+    _need_on(dev, q, kv, scales, out, page_table, seq_lens, sel_idx, sel_counts, scores, lse, ws.buf if ws is not None else None)
     pages, page_size, heads, dim, block = _kv8_geometry(kv, scales)
-    if q.dim() != 3 or q.shape[2] != dim:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim:
         raise RuntimeError(f"q must be [B,Hq,{dim}]")
-    B, Hq, D = q.shape
+    B, Hq, _ = shape
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() == q.data_ptr():
+    elif out.shape != shape or out.dtype != q.dtype or out.data_ptr() == q.data_ptr():
         raise RuntimeError("out must be a tensor of q's shape and dtype, and not q itself")
-    _need_i32("page_table", page_table, B, None)
-    _need_i32("seq_lens", seq_lens, B)
-    a = _lib.AttnKv8Args()
-    a.d_q, a.d_o, a.d_kv, a.d_scales = q.data_ptr(), out.data_ptr(), kv.data_ptr(), scales.data_ptr()
-    if page_table is not None:
-        a.d_page_table, a.page_table_stride = page_table.data_ptr(), page_table.shape[1]
-    else:
-        a.page_table_stride = pages_per_seq if pages_per_seq is not None else pages // max(B, 1)
-    a.d_seq_lens, a.seq_len = _ptr(seq_lens), int(seq_len)
+    _need_vector("seq_lens", seq_lens, B)
+    table, row = _kv8_pages(page_table, pages_per_seq, pages, B)
+    sel_rows = sel_count = score_stride = 0
     if sel_idx is not None:
-        if sel_idx.dim() == 2:
-            _need_i32("sel_idx", sel_idx, B, None)
-            a.sel_rows = 1
-        else:
-            _need_i32("sel_idx", sel_idx, B, Hq, None)
-            a.sel_rows = Hq
-        if sel_counts is not None and (sel_counts.dtype != torch.int32 or sel_counts.numel() != B * a.sel_rows):
-            raise RuntimeError("sel_counts must be int32 with one entry per list")
-        a.d_sel_idx, a.sel_count, a.sel_stride = sel_idx.data_ptr(), sel_idx.shape[-1], sel_idx.shape[-1]
-        a.d_sel_counts = _ptr(sel_counts)
+        lists = sel_idx.shape
+        if sel_idx.dtype != torch.int32 or len(lists) not in (2, 3) or lists[0] != B or (len(lists) == 3 and lists[1] != Hq):
+            raise RuntimeError("sel_idx must be int32 [B,k] or [B,Hq,k]")
+        sel_rows, sel_count = (1 if len(lists) == 2 else Hq), lists[-1]
+        _need_vector("sel_counts", sel_counts, B * sel_rows)
     elif sel_counts is not None:
         raise RuntimeError("sel_counts needs sel_idx")
     if scores is not None:
-        if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[0] != B or scores.shape[1] != Hq:
+        wide = scores.shape
+        if scores.dtype != torch.float32 or len(wide) != 3 or wide[0] != B or wide[1] != Hq:
             raise RuntimeError("scores must be float32 [B,Hq,tokens]")
-        a.d_scores, a.score_stride = scores.data_ptr(), scores.shape[-1]
-    if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (B, Hq):
-            raise RuntimeError("lse must be float32 [B,Hq]")
-        a.d_lse = lse.data_ptr()
-    a.batch, a.num_qo_heads, a.num_kv_heads, a.head_dim = B, Hq, heads, D
-    a.page_size, a.block, a.dtype, a.num_pages, a.sm_scale = page_size, block, _dtype_code(q), pages, float(sm_scale)
-    _launch(lib.tidal_decode_attention_kv8, "tidal_decode_attention_kv8", dev, C.byref(a), ws.buf.data_ptr(), ws.nbytes)
+        score_stride = wide[2]
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq)):
+        raise RuntimeError("lse must be float32 [B,Hq]")
+    a = _lib.AttnKv8Args(q.data_ptr(), out.data_ptr(), kv.data_ptr(), scales.data_ptr(), table, row, _ptr(seq_lens), seq_len,
+                         _ptr(sel_idx), sel_rows, sel_count, sel_count, _ptr(sel_counts), _ptr(scores), score_stride, _ptr(lse),
+                         B, Hq, heads, dim, page_size, block, _dtype_code(q), pages, sm_scale)
+    _launch(lib.tidal_decode_attention_kv8, "tidal_decode_attention_kv8", dev, a, ws.buf.data_ptr(), ws.nbytes)
     return out
 
 
@@ -653,21 +650,18 @@ def accumulate_weights(scores: torch.Tensor, lse: torch.Tensor, weights: torch.T
     """weights[b, j] = decay * weights[b, j] + sum_h exp(scores[b, h, j] - lse[b, h]) for j < the length, in place; see
     tidal_accumulate_weights in include/tidal_b200.h.  scores fp32 [B, heads, >= seq_len] and lse fp32 [B, heads] as a
     selection layer leaves them, weights fp32 [B, >= seq_len]."""
-    dev = scores.device
+    dev = scores.get_device()
     _need_on(dev, scores, lse, weights, seq_lens)
-    if scores.dim() != 3 or scores.dtype != torch.float32:
+    shape = scores.shape
+    if len(shape) != 3 or scores.dtype != torch.float32:
         raise RuntimeError("scores must be float32 [B,heads,tokens] (one row per head)")
-    B, H, n = scores.shape
-    if lse.dtype != torch.float32 or lse.shape != (B, H):
+    B, H, n = shape
+    if _need_rows("lse", lse, B, torch.float32) != H:
         raise RuntimeError("lse must be float32 [B,heads]")
-    if weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[0] != B:
-        raise RuntimeError("weights must be float32 [B,tokens]")
-    _need_i32("seq_lens", seq_lens, B)
-    a = _lib.WeightsArgs()
-    a.d_scores, a.score_stride, a.d_lse = scores.data_ptr(), n, lse.data_ptr()
-    a.d_weights, a.weight_stride = weights.data_ptr(), weights.shape[1]
-    a.d_seq_lens, a.seq_len, a.batch, a.heads, a.decay = _ptr(seq_lens), int(seq_len), B, H, float(decay)
-    _launch(lib.tidal_accumulate_weights, "tidal_accumulate_weights", dev, C.byref(a))
+    columns = _need_rows("weights", weights, B, torch.float32)
+    _need_vector("seq_lens", seq_lens, B)
+    a = _lib.WeightsArgs(scores.data_ptr(), n, lse.data_ptr(), weights.data_ptr(), columns, _ptr(seq_lens), seq_len, B, H, decay)
+    _launch(lib.tidal_accumulate_weights, "tidal_accumulate_weights", dev, a)
     return weights
 
 
@@ -678,28 +672,23 @@ def evict_pages(weights: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
     per token, page_table int32 [rows, >= pages], seq_lens int32 [rows] (at most max_len, default: the columns of
     weights).  Returns (weights, page_table, seq_lens): written to `out`, three tensors of the same shapes that do not
     overlap the inputs, or in place (through a copy of the inputs)."""
-    dev = weights.device
+    dev = weights.get_device()
     _need_on(dev, weights, page_table, seq_lens)
-    if weights.dtype != torch.float32 or weights.dim() != 2:
-        raise RuntimeError("weights must be float32 [rows,tokens]")
     rows = weights.shape[0]
-    _need_i32("page_table", page_table, rows, None)
-    _need_i32("seq_lens", seq_lens, rows)
-    max_len = weights.shape[1] if max_len is None else int(max_len)
-    src = (weights, page_table, seq_lens)
+    columns = _need_rows("weights", weights, rows, torch.float32)
+    pages = _need_rows("page_table", page_table, rows)
+    _need_vector("seq_lens", seq_lens, rows)
     if out is None:
-        src, out = tuple(t.clone() for t in src), src
+        out = weights, page_table, seq_lens
+        weights, page_table, seq_lens = weights.clone(), page_table.clone(), seq_lens.clone()
     else:
         _need_on(dev, *out)
-        if len(out) != 3 or any(o.shape != t.shape or o.dtype != t.dtype for o, t in zip(out, src)):
+        if len(out) != 3 or _need_rows("out[0]", out[0], rows, torch.float32) != columns or _need_rows("out[1]", out[1], rows) != pages:
             raise RuntimeError("out must be (weights, page_table, seq_lens) of the inputs' shapes and types")
-    a = _lib.EvictArgs()
-    a.d_weights, a.d_weights_out, a.weight_stride = src[0].data_ptr(), out[0].data_ptr(), weights.shape[1]
-    a.d_page_table, a.d_page_table_out, a.page_table_stride = src[1].data_ptr(), out[1].data_ptr(), page_table.shape[1]
-    a.d_seq_lens, a.d_seq_lens_out = src[2].data_ptr(), out[2].data_ptr()
-    a.max_len, a.rows, a.page_size, a.keep_pages = max_len, rows, int(page_size), int(keep_pages)
-    a.sink_pages, a.recent_pages = int(sink_pages), int(recent_pages)
-    _launch(lib.tidal_evict_pages, "tidal_evict_pages", dev, C.byref(a))
+        _need_vector("out[2]", out[2], rows)
+    a = _lib.EvictArgs(weights.data_ptr(), out[0].data_ptr(), columns, page_table.data_ptr(), out[1].data_ptr(), pages, seq_lens.data_ptr(),
+                       out[2].data_ptr(), columns if max_len is None else max_len, rows, page_size, keep_pages, sink_pages, recent_pages)
+    _launch(lib.tidal_evict_pages, "tidal_evict_pages", dev, a)
     return out
 
 
