@@ -21,10 +21,12 @@
 // the contraction index and of the output elements is free as long as both operands agree, so the fragments are read
 // 16 bytes at a time, from 16-byte pieces that are permuted within 128 bytes so that no two lanes of an access meet
 // in a bank.  With lane = 4 g + t, a tile of 16 tokens:
-//     S = Q K^T  (M = heads, N = tokens): lane reads 16-byte pieces t, 4 + t of K rows g and 8+g; the four bytes of one
-//                word are elements 2t, 2t+1, 2t+8, 2t+9 of a k-step
-//     O^T = V^T P^T  (M = elements, N = heads): lane reads bytes g*D/8.. of V rows 2t, 2t+1, 2t+8, 2t+9, and the
-//                accumulator of S already has the layout of the B operand P^T
+//     S^T = K Q^T      (M = 16 tokens, N = 8 heads): lane reads 16-byte pieces t and 4 + t of K rows g and 8 + g; the four
+//                      bytes of a word are elements 2t, 2t+1, 2t+8, 2t+9 of a k-step
+//     O^T = V^T P^T    (M = 16 elements, N = 8 heads): lane reads bytes g*D/8.. of V rows 2t, 2t+1, 2t+8, 2t+9; P^T is the
+//                      accumulator of S^T transposed in 8 x 8 blocks (movmatrix)
+// Both products have the few query heads as N: with heads as M (16 rows, most of them zero) the first took twice the
+// instructions and twice the registers.  A lane's accumulators belong to heads 2t and 2t+1 throughout.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -65,11 +67,15 @@ struct AttnKv8Params {
     int32_t ragged;              // lengths differ: 1 = they are added up by every CTA, 2 = a CTA per list
     int32_t tiles_per_list;      // ragged == 0
     int32_t page_shift, block_shift;     // -1 where the size is no power of two
+    int32_t blocks_per_page;
     float sm_scale;
 };
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -79,6 +85,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of 16-bit elements, lane (g, t) holding row g, columns 2t and 2t+1, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // Four e4m3 codes to two fp16 pairs.
 __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& lo, uint32_t& hi) {
@@ -233,13 +245,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
         const int heads = p.per_head ? 1 : min(p.rows, (kvh + 1) * p.G - hq0);         // query heads of this unit
         const int seq = p.seq_lens ? max(0, min(p.seq_lens[b], p.seq_len)) : p.seq_len;
 
-        // ---- Q fragments, scaled to [2^11, 2^12) per head
+        // ---- Q fragments (lane: head g of each eight), scaled to [2^11, 2^12) per head
         uint32_t qa[NR][KS][2], ql[QS ? NR : 1][QS ? KS : 1][2];
-        float qn[NR], qn2[NR];                                           // undo the scaling and apply sm_scale (in log2 units)
+        float qn[NR][2], qn2[NR][2];                                     // of heads 2t, 2t+1: undo the scaling and apply sm_scale (qn2 in log2 units)
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int row = g + 8 * r;
-            const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)b * p.Hq + hq0 + (row < heads ? row : 0)) * D;
+            const int head = g + 8 * r;
+            const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)b * p.Hq + hq0 + (head < heads ? head : 0)) * D;
             float f[KS][4], top = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -255,24 +267,31 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             int sh = 138 - (int)(__float_as_uint(top) >> 23);           // 11 less the exponent of the largest element
             sh = top == 0.f ? 0 : min(sh, 120);
             const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-            qn[r] = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
-            qn2[r] = qn[r] * kLog2e;
+            const float down = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                qn[r][e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
+                qn2[r][e] = qn[r][e] * kLog2e;
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float x0 = f[ks][2 * i] * up, x1 = f[ks][2 * i + 1] * up;
-                    qa[r][ks][i] = row < heads ? pack_f16(x0, x1) : 0u;
-                    if (QS) ql[QS ? r : 0][QS ? ks : 0][i] = row < heads ? pack_f16_rest(x0, x1, qa[r][ks][i]) : 0u;
+                    qa[r][ks][i] = head < heads ? pack_f16(x0, x1) : 0u;
+                    if (QS) ql[QS ? r : 0][QS ? ks : 0][i] = head < heads ? pack_f16_rest(x0, x1, qa[r][ks][i]) : 0u;
                 }
         }
 
-        float o[NR][KS][4];
-        float m[NR], M[NR], l[NR];
+        float o[NR][KS][4];                                              // [eight heads][16 elements]: elements 2j, 2j+1 of g*D/8.., heads 2t, 2t+1
+        float m[NR][2], M[NR][2], l[NR][2];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            m[r] = M[r] = -FLT_MAX;
-            l[r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[r][e] = M[r][e] = -FLT_MAX;
+                l[r][e] = 0.f;
+            }
 #pragma unroll
             for (int j = 0; j < KS; ++j)
 #pragma unroll
@@ -281,23 +300,29 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
 
         // ---- looking tokens up: lane i follows token i of a pair of tiles; its list entry is loaded two pairs ahead of
         //      its copies, its page one pair ahead, its scales with the copies
-        const size_t pitch = (size_t)p.Hkv * D;
-        const int ps = p.map.page_size;
         constexpr int PR = D / 16, TI = 32 / PR;                          // 16-byte pieces of a row; tokens that one copy of the warp covers
         const int c_tok = lane / PR, c_piece = lane % PR;
+        const int ps = p.map.page_size;
+        const uint32_t pitch = (uint32_t)p.Hkv * D;
         const uint8_t* k_src = p.kv + (size_t)kvh * D + c_piece * 16;
-        const size_t v_plane = (size_t)ps * pitch;
+        const uint8_t* v_src = k_src + (size_t)ps * pitch;
+        const uint32_t ring_k = smem_u32(ring) + k_piece<D>(c_tok, c_piece), ring_v = smem_u32(ring) + kKv8Tile * D + v_piece<D>(c_tok, c_piece);
         const int k_off = k_piece<D>(g, t), v_off = v_piece<D>(2 * t, g * VB / 16) + (g * VB & 15);
         const int v_off1 = v_piece<D>(2 * t + 1, g * VB / 16) + (g * VB & 15);
+        const int32_t* sel = p.sel_idx ? p.sel_idx + (size_t)list * p.sel_stride : nullptr;
+        const int32_t* table = p.map.page_table ? p.map.page_table + (size_t)b * p.map.pt_stride : nullptr;
+        const int page0 = (int)((int64_t)b * p.map.pt_stride);           // without a table
+        const uint8_t* sc_src = p.scales + kvh;
+        const uint32_t sc_plane = (uint32_t)p.blocks_per_page * p.Hkv;
         auto fetch_pos = [&](int pair) -> int {
             const int i = w0 + pair * TT + lane;
             if (pair >= n_pairs || i >= tok1) return INT_MIN;            // no token here
-            return p.sel_idx ? max(p.sel_idx[(size_t)list * p.sel_stride + i], -1) : i;
+            return sel ? max(sel[i], -1) : i;
         };
+        auto page_of = [&](int pos) -> int { return p.page_shift >= 0 ? pos >> p.page_shift : pos / ps; };
         auto fetch_page = [&](int pos) -> int {
             if (pos < 0 || pos >= seq) return -1;
-            const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / ps;
-            return p.map.page_table ? p.map.page_table[(size_t)b * p.map.pt_stride + pg] : (int)((int64_t)b * p.map.pt_stride + pg);
+            return table ? table[page_of(pos)] : page0 + page_of(pos);
         };
         int pos_c = fetch_pos(0), page_c = fetch_page(pos_c), pos_n = fetch_pos(1);
         int row = -1;                                                    // pool row of the lane's K row (its V row lies ps rows further), or -1
@@ -305,15 +330,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
         uint32_t full = 0;                                               // bit i: every token of the pair issued i pairs ago is there
         auto look_up = [&](int pair) {
             row = -1;
-            if (page_c >= 0 && page_c < p.map.num_pages) {
-                const int pg = p.page_shift >= 0 ? pos_c >> p.page_shift : pos_c / ps;
-                const int entry = pos_c - pg * ps;
+            if (page_c >= 0 && page_c < (int)p.map.num_pages) {
+                const int entry = pos_c - page_of(pos_c) * ps;
                 row = page_c * 2 * ps + entry;
-                const int blk = p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block;
-                const int per_page = p.block_shift >= 0 ? ps >> p.block_shift : ps / p.block;
-                const uint8_t* at = p.scales + ((size_t)page_c * 2 * per_page + blk) * p.Hkv + kvh;
-                sc_k = at[0];
-                sc_v = at[(size_t)per_page * p.Hkv];
+                uint32_t at = (uint32_t)page_c * 2u * sc_plane;          // scale bytes number less than 2^32, checked on the host
+                if (p.blocks_per_page > 1) at += (uint32_t)(p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block) * (uint32_t)p.Hkv;
+                sc_k = sc_src[at];
+                sc_v = sc_src[at + sc_plane];
             } else if (pos_c != INT_MIN) {
                 atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
             }
@@ -325,19 +348,26 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
         auto park_scales = [&](int pair) {
             sc_ring[warp][pair & (NP - 1)][lane] = row >= 0 ? make_float2(scale_value(sc_k), sc_v ? (float)((int)sc_v - 127) : -INFINITY) : make_float2(-1.f, -INFINITY);
         };
-        auto copy = [&](int it, unsigned char* dst) {
+        auto copy = [&](int it, uint32_t slot) {
             const int l0 = (it & 1) * kKv8Tile + c_tok;
-            const bool all = full & 1u;
+            if (full & 1u) {
 #pragma unroll
-            for (int i = 0; i < kKv8Tile / TI; ++i) {
-                const int r = __shfl_sync(0xffffffffu, row, l0 + i * TI);
-                const uint8_t* src = k_src + (all ? (uint32_t)r : (uint32_t)max(r, 0)) * pitch;
-                cp_async16(dst + k_piece<D>(i * TI + c_tok, c_piece), src, all || r >= 0);
-                cp_async16(dst + kKv8Tile * D + v_piece<D>(i * TI + c_tok, c_piece), src + v_plane, all || r >= 0);
+                for (int i = 0; i < kKv8Tile / TI; ++i) {
+                    const uint32_t r = (uint32_t)__shfl_sync(0xffffffffu, row, l0 + i * TI);
+                    cp_async16(ring_k + slot + i * 512, k_src + (uint64_t)r * pitch);
+                    cp_async16((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + (uint64_t)r * pitch);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kKv8Tile / TI; ++i) {
+                    const int r = __shfl_sync(0xffffffffu, row, l0 + i * TI);
+                    const uint64_t at = (uint64_t)max(r, 0) * pitch;
+                    cp_async16_or_zero(ring_k + slot + i * 512, k_src + at, r >= 0);
+                    cp_async16_or_zero((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + at, r >= 0);
+                }
             }
         };
 
-        int put_slot = 0, use_slot = 0;
 #pragma unroll
         for (int s = 0; s < S - 1; ++s) {
             if (s < n_it) {
@@ -345,123 +375,134 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                     look_up(s >> 1);
                     park_scales(s >> 1);
                 }
-                copy(s, ring + s * Kv8Ring<D>::stage_bytes);
+                copy(s, s * Kv8Ring<D>::stage_bytes);
             }
             cp_async_commit();
         }
-        put_slot = S - 1;
+        uint32_t put_slot = (S - 1) * Kv8Ring<D>::stage_bytes, use_slot = 0;
         for (int it = 0; it < n_it; ++it) {
             const int ahead = it + S - 1;
             const bool looked = ahead < n_it && (ahead & 1) == 0;
             if (looked) look_up(ahead >> 1);
-            if (ahead < n_it) copy(ahead, ring + put_slot * Kv8Ring<D>::stage_bytes);
-            put_slot = put_slot == S - 1 ? 0 : put_slot + 1;
+            if (ahead < n_it) copy(ahead, put_slot);
+            put_slot = put_slot == (S - 1) * Kv8Ring<D>::stage_bytes ? 0 : put_slot + Kv8Ring<D>::stage_bytes;
             cp_async_commit();
             cp_async_wait<S - 1>();
             __syncwarp();
-            const unsigned char* st = ring + use_slot * Kv8Ring<D>::stage_bytes;
-            use_slot = use_slot == S - 1 ? 0 : use_slot + 1;
-            // ---- S = Q K^T
-            float sf[2][4];
+            const unsigned char* st = ring + use_slot;
+            use_slot = use_slot == (S - 1) * Kv8Ring<D>::stage_bytes ? 0 : use_slot + Kv8Ring<D>::stage_bytes;
+            // ---- S^T = K Q^T: tokens g and 8 + g, heads 2t and 2t+1
+            float sf[NR][4];
 #pragma unroll
-            for (int n2 = 0; n2 < 2; ++n2) {
+            for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sf[n2][i] = 0.f;
+                for (int i = 0; i < 4; ++i) sf[r][i] = 0.f;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const uint4 kw = *reinterpret_cast<const uint4*>(st + n2 * 8 * D + (k_off ^ c * 64));
-                    const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+            for (int c = 0; c < KC; ++c) {
+                const uint4 k0 = *reinterpret_cast<const uint4*>(st + (k_off ^ c * 64)), k1 = *reinterpret_cast<const uint4*>(st + 8 * D + (k_off ^ c * 64));
+                const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t b0, b1;
-                        halves_of(w[i], b0, b1);
-                        const int ks = c * 4 + i;
-                        mma_f16(sf[n2], qa[0][ks][0], R2 ? qa[NR - 1][ks][0] : 0u, qa[0][ks][1], R2 ? qa[NR - 1][ks][1] : 0u, b0, b1);
-                        if (QS) mma_f16(sf[n2], ql[0][QS ? ks : 0][0], R2 ? ql[QS ? NR - 1 : 0][QS ? ks : 0][0] : 0u, ql[0][QS ? ks : 0][1],
-                                        R2 ? ql[QS ? NR - 1 : 0][QS ? ks : 0][1] : 0u, b0, b1);
+                for (int i = 0; i < 4; ++i) {
+                    const int ks = c * 4 + i;
+                    uint32_t a[4];
+                    halves_of(lo[i], a[0], a[2]);
+                    halves_of(hi[i], a[1], a[3]);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        mma_f16(sf[r], a[0], a[1], a[2], a[3], qa[r][ks][0], qa[r][ks][1]);
+                        if (QS) mma_f16(sf[r], a[0], a[1], a[2], a[3], ql[QS ? r : 0][QS ? ks : 0][0], ql[QS ? r : 0][QS ? ks : 0][1]);
                     }
                 }
             }
-            // ---- scales of this lane's four tokens (2t, 2t+1, 8+2t, 9+2t)
-            const float2* scp = &sc_ring[warp][(it >> 1) & (NP - 1)][(it & 1) * kKv8Tile + 2 * t];
-            const float4 s01 = *reinterpret_cast<const float4*>(scp), s23 = *reinterpret_cast<const float4*>(scp + 8);
-            const float kf[4] = {s01.x, s01.z, s23.x, s23.z}, ev[4] = {s01.y, s01.w, s23.y, s23.w};
+            // ---- scales of the two tokens; value i of a lane: token g + 8 (i / 2), head 2t + i % 2
+            const float2* scp = &sc_ring[warp][(it >> 1) & (NP - 1)][(it & 1) * kKv8Tile + g];
+            const float2 s0 = scp[0], s1 = scp[8];
+            const float kf[2] = {s0.x, s1.x}, ev[2] = {s0.y, s1.y};
             // the pair of tile `it` was looked up ((ahead or the last tile) / 2 - it / 2) pairs before the newest one
             const bool all = full >> ((min(ahead, n_it - 1) >> 1) - (it >> 1)) & 1u;
             if (p.scores) {
-                const int i0 = w0 + (it >> 1) * TT + (it & 1) * kKv8Tile + 2 * t;      // list index of the lane's first token
+                const int i0 = w0 + (it >> 1) * TT + (it & 1) * kKv8Tile + g;          // list index of the lane's first token
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
-                    if (g + 8 * r < heads) {
-                        float* at = p.scores + ((size_t)b * p.Hq + hq0 + g + 8 * r) * p.score_stride + i0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (kf[i] >= 0.f) at[(i >> 1) * 8 + (i & 1)] = sf[i >> 1][2 * r + (i & 1)] * kf[i] * qn[r];
-                    }
-            }
-            // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M + 14 for the weights
-            uint32_t pb[NR][2], pl[PS ? NR : 1][2];
-            float xl[NR][4], xw[NR][4];
-            auto exponents = [&]() -> bool {
-                bool moved = false;
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float f = kf[i] * qn2[r], y = sf[i >> 1][2 * r + (i & 1)];
-                        xl[r][i] = fmaf(y, f, -m[r]);
-                        xw[r][i] = fmaf(y, f, ev[i] - M[r]);
-                        if (!all && kf[i] < 0.f) xl[r][i] = -INFINITY;
+                        const int head = 2 * t + (i & 1) + 8 * r;
+                        if (head < heads && kf[i >> 1] >= 0.f)
+                            p.scores[((size_t)b * p.Hq + hq0 + head) * p.score_stride + i0 + (i >> 1) * 8] = sf[r][i] * kf[i >> 1] * qn[r][i & 1];
                     }
-                    moved |= fmaxf(fmaxf(xl[r][0], xl[r][1]), fmaxf(xl[r][2], xl[r][3])) > 0.f ||
-                             fmaxf(fmaxf(xw[r][0], xw[r][1]), fmaxf(xw[r][2], xw[r][3])) > 14.f;
+            }
+            // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M for the weights (M is kept less
+            //      the 14 binades of the weights' range)
+            float xl[NR][4], xw[NR][4];
+            auto exponents = [&]() -> bool {
+                float top = 0.f, topw = 14.f;
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = kf[i >> 1] * qn2[r][i & 1];
+                        xl[r][i] = fmaf(sf[r][i], f, -m[r][i & 1]);
+                        xw[r][i] = fmaf(sf[r][i], f, ev[i >> 1] - M[r][i & 1]);
+                    }
+                if (!all) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) xl[r][i] = kf[i >> 1] < 0.f ? -INFINITY : xl[r][i];
                 }
-                return moved;
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        top = fmaxf(top, xl[r][i]);
+                        topw = fmaxf(topw, xw[r][i]);
+                    }
+                return top > 0.f || topw > 14.f;
             };
             if (__any_sync(0xffffffffu, exponents())) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float top = -FLT_MAX, topv = -FLT_MAX;
+                for (int r = 0; r < NR; ++r)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (kf[i] >= 0.f) {
-                            const float x = sf[i >> 1][2 * r + (i & 1)] * (kf[i] * qn2[r]);
-                            top = fmaxf(top, x);
-                            topv = fmaxf(topv, x + ev[i]);
+                    for (int e = 0; e < 2; ++e) {
+                        float top = -FLT_MAX, topv = -FLT_MAX;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (kf[i] >= 0.f) {
+                                const float x = sf[r][2 * i + e] * (kf[i] * qn2[r][e]);
+                                top = fmaxf(top, x);
+                                topv = fmaxf(topv, x + ev[i]);
+                            }
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                            topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
                         }
+                        const float mn = fmaxf(m[r][e], ceilf(top)), Mn = fmaxf(M[r][e], ceilf(topv) - 14.f);
+                        l[r][e] *= fast_exp2(m[r][e] - mn);
+                        const float a = fast_exp2(M[r][e] - Mn);
+                        m[r][e] = mn;
+                        M[r][e] = Mn;
 #pragma unroll
-                    for (int off = 1; off < 4; off <<= 1) {
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                        topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
+                        for (int j = 0; j < KS; ++j) {
+                            o[r][j][e] *= a;
+                            o[r][j][2 + e] *= a;
+                        }
                     }
-                    // M is kept less the 14 of the weights' range
-                    const float mn = fmaxf(m[r], ceilf(top)), Mn = fmaxf(M[r], ceilf(topv) - 14.f);
-                    l[r] *= fast_exp2(m[r] - mn);
-                    const float a = fast_exp2(M[r] - Mn);
-                    m[r] = mn;
-                    M[r] = Mn;
-                    const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
-#pragma unroll
-                    for (int j = 0; j < KS; ++j) {
-                        o[r][j][0] *= a0;
-                        o[r][j][1] *= a1;
-                        o[r][j][2] *= a0;
-                        o[r][j][3] *= a1;
-                    }
-                }
                 exponents();
             }
+            uint32_t pb[NR][2], pl[PS ? NR : 1][2];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 float w[4];
-                l[r] += (fast_exp2(xl[r][0]) + fast_exp2(xl[r][1])) + (fast_exp2(xl[r][2]) + fast_exp2(xl[r][3]));
+                l[r][0] += fast_exp2(xl[r][0]) + fast_exp2(xl[r][2]);
+                l[r][1] += fast_exp2(xl[r][1]) + fast_exp2(xl[r][3]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = fast_exp2(xw[r][i]);
-                pb[r][0] = pack_f16(w[0], w[1]);
-                pb[r][1] = pack_f16(w[2], w[3]);
-                if (PS) {
-                    pl[PS ? r : 0][0] = pack_f16_rest(w[0], w[1], pb[r][0]);
-                    pl[PS ? r : 0][1] = pack_f16_rest(w[2], w[3], pb[r][1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
+                    pb[r][i] = transpose8x8(hi);
+                    if (PS) pl[PS ? r : 0][i] = transpose8x8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi));
                 }
             }
             // ---- O^T += V^T P^T
@@ -502,23 +543,24 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
         __syncthreads();
         float* so = reinterpret_cast<float*>(smem);                      // [warps][rows][D]
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (t == 0) {
-                ml[warp][g + 8 * r][0] = m[r];
-                ml[warp][g + 8 * r][1] = l[r];
-            }
-            const float f = fast_exp2(M[r] - m[r]);
-            const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const int h0 = 2 * t + 8 * r;
-                float* at = so + ((size_t)warp * p.rows + h0) * D + g * VB + 2 * j;
-                if (h0 < p.rows) *reinterpret_cast<float2*>(at) = make_float2(o[r][j][0] * f0, o[r][j][2] * f0);
-                if (h0 + 1 < p.rows) *reinterpret_cast<float2*>(at + D) = make_float2(o[r][j][1] * f1, o[r][j][3] * f1);
+            for (int e = 0; e < 2; ++e) {
+                const int head = 2 * t + e + 8 * r;
+                float sum = l[r][e];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                if (g == 0) {
+                    ml[warp][head][0] = m[r][e];
+                    ml[warp][head][1] = sum;
+                }
+                if (head < p.rows) {
+                    const float f = fast_exp2(M[r][e] - m[r][e]);
+                    float* at = so + ((size_t)warp * p.rows + head) * D + g * VB;
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(o[r][j][e] * f, o[r][j][2 + e] * f);
+                }
             }
-        }
         __syncthreads();
         const int unit_rows = p.HC * p.rows, vecs = unit_rows * (D / 4);
         const size_t part0 = (size_t)slice * (p.ctas + p.lists);
@@ -621,6 +663,7 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     TIDAL_REQUIRE(a->block >= 1 && a->page_size % a->block == 0, TIDAL_ERR_ARG, "block %d does not divide page_size %d", a->block, a->page_size);
     TIDAL_REQUIRE(a->seq_len >= 0, TIDAL_ERR_ARG, "negative seq_len");
     TIDAL_REQUIRE(a->num_pages * 2 * a->page_size < ((int64_t)1 << 31), TIDAL_ERR_ARG, "the pool has 2^31 token rows or more (num_pages * 2 * page_size)");
+    TIDAL_REQUIRE(a->num_pages * 2 * (a->page_size / a->block) * a->num_kv_heads < ((int64_t)1 << 32), TIDAL_ERR_ARG, "the pool has 2^32 scales or more");
     const bool sel = a->d_sel_idx != nullptr;
     if (sel) {
         TIDAL_REQUIRE(a->sel_rows == 1 || a->sel_rows == a->num_qo_heads, TIDAL_ERR_ARG, "sel_rows must be 1 or num_qo_heads, got %d", a->sel_rows);
@@ -652,6 +695,7 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     auto shift_of = [](int x) { return (x & (x - 1)) == 0 ? 31 - __builtin_clz((unsigned)x) : -1; };
     p.page_shift = shift_of(a->page_size);
     p.block_shift = shift_of(a->block);
+    p.blocks_per_page = a->page_size / a->block;
     p.per_head = p.sel_rows != 1;
     const int64_t lists = (int64_t)a->batch * p.sel_rows;
     TIDAL_REQUIRE(lists <= 1 << 20, TIDAL_ERR_ARG, "attention_kv8: more than 2^20 token lists");
