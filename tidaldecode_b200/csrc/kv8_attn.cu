@@ -167,11 +167,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int TG = kKv8Warps / p.HC, TT = 2 * kKv8Tile * TG;
     const int uw = warp % p.HC, tg = warp / p.HC;
-    const int cta = blockIdx.x, slice = blockIdx.y;
+    const int cta = blockIdx.y, slice = blockIdx.x;
     unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D>::stage_bytes;
 
+    if (tid == 0) TIDAL_STAMP(0);
     pdl_wait();
     pdl_launch_dependents();
+    if (tid == 0) TIDAL_STAMP(1);
 
     // ---- this CTA's range of tiles
     int64_t tile, tile_end;
@@ -389,6 +391,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             cp_async_commit();
             cp_async_wait<S - 1>();
             __syncwarp();
+            if (tid == 0 && it == 0) TIDAL_STAMP(2);
             const unsigned char* st = ring + use_slot;
             use_slot = use_slot == (S - 1) * Kv8Ring<D>::stage_bytes ? 0 : use_slot + Kv8Ring<D>::stage_bytes;
             // ---- S^T = K Q^T: tokens g and 8 + g, heads 2t and 2t+1
@@ -538,6 +541,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             __syncwarp();                                                // the tile's slot is the next to be filled
         }
         cp_async_wait<0>();
+        if (tid == 0) TIDAL_STAMP(3);
 
         // ---- warps of a unit merge through shared memory: o relative to m
         __syncthreads();
@@ -630,6 +634,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             }
         }
         __syncthreads();                                                 // the ring is free for the next segment
+        if (tid == 0) TIDAL_STAMP(4);
         tile = seg_end;
         if (p.ragged == 2) break;
     }
@@ -640,7 +645,7 @@ static int launch_attn_kv8(const AttnKv8Params& p, cudaStream_t st) {
     const size_t smem = Kv8Ring<D>::bytes + (p.ragged == 1 ? sizeof(int) * (p.lists + 1) : 0);
     auto go = [&](auto kern) -> int {
         TIDAL_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        TIDAL_CUDA_OK(launch_pdl(kern, dim3(p.ctas, p.slices), dim3(kKv8Warps * 32), smem, st, 1, p));
+        TIDAL_CUDA_OK(launch_pdl(kern, dim3(p.slices, p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
         count_launch();
         return TIDAL_OK;
     };
@@ -704,7 +709,8 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     p.groups = (G + 15) / 16;
     p.rows = (G + p.groups - 1) / p.groups;
     const int units = p.per_head ? 1 : p.Hkv * p.groups;
-    p.HC = 1;
+    // two units to a CTA where there is work for every SM: rows of two heads are adjacent (104 us instead of 111 for 512 MB)
+    p.HC = units % 2 == 0 && lists * units * (int64_t)ntok >= (int64_t)1 << 18 ? 2 : 1;
     p.slices = units / p.HC;
     const int TT = 2 * kKv8Tile * (kKv8Warps / p.HC);
     const bool ragged = sel ? p.sel_counts != nullptr : p.seq_lens != nullptr;
@@ -729,3 +735,5 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
         default: return wide ? launch_attn_kv8<float, 128>(p, st) : launch_attn_kv8<float, 64>(p, st);
     }
 }
+
+TIDAL_TRACE_READER(tidal_trace_read_kv8)
