@@ -1,5 +1,7 @@
 // Bounding a cache by what its tokens have been worth: softmax weights of a selection layer added up per token, and the
 // pages of least weight moved out of a page table.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace tidal {
@@ -44,111 +46,241 @@ struct EvictParams {
     const int32_t* seq_lens;
     int32_t* seq_lens_out;
     int32_t max_len, page_size, keep, sink, recent;
+    int32_t cached;              // page keys are kept in shared memory
+    int32_t row_vec4, table_vec4;// rows of weights / of the table start on 16 bytes
+    int32_t vec4;                // ... and so do the pages of weights
+    int32_t page_shift;          // of page_size, or of page_size / 4 with vec4; -1: no power of two
 };
 
 // Order-preserving key of a weight (see ordered_key); the two zeros are equal, every NaN is the greatest.
 __device__ __forceinline__ uint32_t weight_key(float x) { return x != x ? 0xffffffffu : ordered_key(x + 0.f); }
 // Key of page pg of a row of `len` tokens.
-__device__ __forceinline__ uint32_t page_key(const float* w, int pg, int page_size, int len) {
+__device__ __forceinline__ uint32_t page_key(const float* w, int pg, int page_size, int len, bool vec4) {
     if (page_size == 1) return weight_key(w[pg]);
     const int t0 = pg * page_size, t1 = (int)min((int64_t)t0 + page_size, (int64_t)len);
     double sum = 0.0;
-    for (int t = t0; t < t1; ++t) sum += (double)w[t];
+    int t = t0;
+    if (vec4)
+        for (; t + 4 <= t1; t += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(w + t);
+            sum += ((double)v.x + (double)v.y) + ((double)v.z + (double)v.w);
+        }
+    for (; t < t1; ++t) sum += (double)w[t];
     return weight_key((float)sum);
 }
 
-// Exclusive prefix over the CTA of a 0/1 flag per thread; *total receives the CTA's sum.  Every thread calls it.
-__device__ __forceinline__ int block_rank(bool flag, int* total, int* warp_sums) {
-    const uint32_t m = __ballot_sync(0xffffffffu, flag);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    __syncthreads();
-    if (lane == 0) warp_sums[warp] = __popc(m);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < warps; ++i) {
-        const int c = warp_sums[i];
-        before += i < warp ? c : 0;
-        all += c;
+// Inclusive prefix over the CTA's threads; `sums` holds one word per warp.  Every thread calls it.
+__device__ __forceinline__ int block_inclusive(int x, int* sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
     }
-    *total = all;
-    return before + __popc(m & ((1u << lane) - 1u));
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    int s = sums[lane];                                          // 32 warps
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, off);
+        if (lane >= off) s += y;
+    }
+    return x + (warp > 0 ? __shfl_sync(0xffffffffu, s, warp - 1) : 0);
 }
 
-// One CTA per row.  The keep - sink - recent heaviest of the pages between the protected ones are found by a radix
-// select over their keys, four digits of eight bits from the top; equal keys at the threshold go to the lower pages.
-// Then one walk over the pages in order gives every page its place.
-__global__ void __launch_bounds__(1024) evict_pages_kernel(const EvictParams p) {
-    __shared__ uint32_t hist[256];
-    __shared__ int warp_sums[32];
-    __shared__ uint32_t s_digit;
-    __shared__ int s_need;
+// dst[i] = src[i] (src NULL: 0) for from <= i < to, by threads me of `all`; vec4: dst and src start on 16 bytes, and the
+// vectors that lie in the range whole go as such.  Out of line: it is called in several places of a kernel whose
+// instructions are fetched cold.
+static __device__ __noinline__ void copy_row(uint32_t* dst, const uint32_t* src, uint32_t from, uint32_t to, uint32_t me, uint32_t all, bool vec4) {
+    if (vec4) {
+        const uint32_t a = min((from + 3) / 4, (to + 3) / 4), b = max(to / 4, a);
+        if (me < a * 4 - from && from + me < to) dst[from + me] = src ? src[from + me] : 0u;
+#pragma unroll 4
+        for (uint32_t v = a + me; v < b; v += all) reinterpret_cast<uint4*>(dst)[v] = src ? reinterpret_cast<const uint4*>(src)[v] : make_uint4(0, 0, 0, 0);
+        from = max(b * 4, from);
+    }
+    for (uint32_t k = from + me; k < to; k += all) dst[k] = src ? src[k] : 0u;
+}
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictBins = 2048;          // 11-bit digits, from the top: 11 + 11 + 10 bits
+constexpr int kEvictKeys = 48 * 1024;     // page keys a CTA keeps in shared memory; beyond that they are formed anew
+
+// A cluster per row, each of its CTAs with a contiguous part of the row's pages.  The keep - sink - recent heaviest of the
+// pages between the protected ones are found by a radix select over their keys: a histogram per CTA and digit, added up
+// through distributed shared memory by every CTA, so that all know the threshold after one cluster barrier per digit.
+// Equal keys at the threshold go to the lower pages.  A warp owns 32-page groups in order; two walks over them (count,
+// then place) with one prefix over the warps and one over the CTAs between them give every page its place.
+// Bound by latency: three histogram passes and four cluster barriers; the bytes are nothing beside them.
+__global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictParams p) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint32_t keys[];
+    __shared__ uint32_t hist[3][kEvictBins];
+    __shared__ int sums[32], s_pick[2], s_ties, s_more;
+    __shared__ int warp_ties[32], warp_more[32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
     pdl_wait();
     pdl_launch_dependents();
-    const int row = blockIdx.x;
+    const int row = blockIdx.x / C;
     const float* w = p.weights + (size_t)row * p.weight_stride;
     float* w_out = p.weights_out + (size_t)row * p.weight_stride;
     const int32_t* table = p.table + (size_t)row * p.table_stride;
     int32_t* table_out = p.table_out + (size_t)row * p.table_stride;
     const int len = p.seq_lens ? max(0, min(p.seq_lens[row], p.max_len)) : p.max_len;
-    const int used = (int)(((int64_t)len + p.page_size - 1) / p.page_size);
-    const int max_pages = (int)(((int64_t)p.max_len + p.page_size - 1) / p.page_size);
-    const int tid = threadIdx.x, nt = blockDim.x;
-    if (used <= p.keep) {
-        for (int i = tid; i < max_pages; i += nt) table_out[i] = table[i];
-        for (int i = tid; i < p.max_len; i += nt) w_out[i] = w[i];
-        if (tid == 0) p.seq_lens_out[row] = len;
+    const int ps = p.page_size;
+    const int used = (int)(((int64_t)len + ps - 1) / ps);
+    const int max_pages = (int)(((int64_t)p.max_len + ps - 1) / ps);
+    const uint32_t me = (uint32_t)(rank * kEvictThreads + tid), all = (uint32_t)(C * kEvictThreads);
+    if (used <= p.keep) {                                        // the whole cluster agrees
+        copy_row((uint32_t*)table_out, (const uint32_t*)table, 0, max_pages, me, all, p.table_vec4 != 0);
+        copy_row((uint32_t*)w_out, (const uint32_t*)w, 0, p.max_len, me, all, p.row_vec4 != 0);
+        if (me == 0) p.seq_lens_out[row] = len;
         return;
     }
+    const int new_len = len - (used - p.keep) * ps;
+    copy_row((uint32_t*)table_out, (const uint32_t*)table, used, max_pages, me, all, p.table_vec4 != 0);
+    copy_row((uint32_t*)w_out, nullptr, new_len, len, me, all, p.row_vec4 != 0);
+    copy_row((uint32_t*)w_out, (const uint32_t*)w, len, p.max_len, me, all, p.row_vec4 != 0);
+    if (me == 0) p.seq_lens_out[row] = new_len;
+
+    // ---- this CTA's pages [base, base + n), and of each warp the 32-page groups [g0, g1) of them
+    const int groups = (used + 31) / 32, per_cta = (groups + C - 1) / C;
+    const int base = min(rank * per_cta, groups) * 32, n = min(used - base, per_cta * 32);
+    const int mine = n > 0 ? (n + 31) / 32 : 0, per_warp = (mine + 31) / 32;
+    const int g0 = min(warp * per_warp, mine), g1 = min(g0 + per_warp, mine);
     const int lo = p.sink, hi = used - p.recent;                 // the pages that compete
-    int need = p.keep - p.sink - p.recent;                       // of them stay
-    uint32_t prefix = 0;                                         // the threshold key, digit by digit
-    if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += nt) hist[i] = 0;
-            __syncthreads();
-            for (int i = lo + tid; i < hi; i += nt) {
-                const uint32_t k = page_key(w, i, p.page_size, len);
-                if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[k >> shift & 255u], 1u);
+    const int places = p.keep - p.sink - p.recent;               // of them stay
+    const bool cached = p.cached != 0;
+    const bool vec4 = p.vec4 != 0;
+    auto key_of = [&](int i) -> uint32_t { return cached ? keys[i] : page_key(w, base + i, ps, len, vec4); };
+    if (cached)
+#pragma unroll 4
+        for (int i = tid; i < n; i += kEvictThreads) keys[i] = page_key(w, base + i, ps, len, vec4);
+    __syncthreads();
+
+    uint32_t threshold = 0;
+    int need = places;                                           // how many of the keys with the threshold's leading digits stay
+    if (places > 0) {
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+            const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
+            for (int i = tid; i < n; i += kEvictThreads) {
+                const int pg = base + i;
+                const uint32_t k = key_of(i);
+                if (pg >= lo && pg < hi && (d == 0 || k >> (shift + bits) == threshold >> (shift + bits)))
+                    atomicAdd(&hist[d][k >> shift & ((1u << bits) - 1u)], 1u);
+            }
+            if (C > 1) cluster.sync();
+            else __syncthreads();
+            // thread t takes the bins 2047 - 2t and 2046 - 2t: a prefix over the threads counts from the greatest key down
+            const int bin = kEvictBins - 2 - 2 * tid;
+            int c0 = 0, c1 = 0;
+            for (int r = 0; r < C; ++r) {
+                const uint2 v = *reinterpret_cast<const uint2*>((C > 1 ? cluster.map_shared_rank(&hist[d][0], r) : &hist[d][0]) + bin);
+                c0 += (int)v.x;
+                c1 += (int)v.y;
+            }
+            const int upto = block_inclusive(c0 + c1, sums), before = upto - c0 - c1;
+            if (before < need && need <= upto) {                 // exactly one thread: there are at least `need` such keys
+                const bool high = need <= before + c1;
+                s_pick[0] = bin + (high ? 1 : 0);
+                s_pick[1] = need - before - (high ? 0 : c1);
             }
             __syncthreads();
-            if (tid == 0) {
-                int left = need, d = 255;
-                while (d > 0 && (int)hist[d] < left) left -= (int)hist[d--];
-                s_digit = (uint32_t)d;
-                s_need = left;
+            threshold |= (uint32_t)s_pick[0] << shift;
+            need = s_pick[1];
+        }
+    }
+
+    // ---- first walk: how many of each warp's pages lie above the threshold (or are protected), how many at it
+    auto classify = [&](int gr, bool* in, bool* tie) -> bool {
+        const int i = gr * 32 + lane, pg = base + i;
+        *in = i < n;
+        const bool competes = *in && pg >= lo && pg < hi;
+        const uint32_t k = competes ? key_of(i) : 0u;
+        *tie = competes && places > 0 && k == threshold;
+        return *in && (!competes || (places > 0 && k > threshold));
+    };
+    int ties = 0, more = 0;
+    for (int gr = g0; gr < g1; ++gr) {
+        bool in, tie;
+        const bool above = classify(gr, &in, &tie);
+        more += __popc(__ballot_sync(0xffffffffu, above));
+        ties += __popc(__ballot_sync(0xffffffffu, tie));
+    }
+    if (lane == 0) warp_ties[warp] = ties, warp_more[warp] = more;
+    __syncthreads();
+    if (warp == 0) {
+        int a = warp_ties[lane], b = warp_more[lane];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, a, off), z = __shfl_up_sync(0xffffffffu, b, off);
+            if (lane >= off) a += y, b += z;
+        }
+        if (lane == 31) s_ties = a, s_more = b;
+        const int ta = __shfl_up_sync(0xffffffffu, a, 1), tb = __shfl_up_sync(0xffffffffu, b, 1);
+        warp_ties[lane] = lane > 0 ? ta : 0;
+        warp_more[lane] = lane > 0 ? tb : 0;
+    }
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    int tie_at = warp_ties[warp], more_at = warp_more[warp];     // ties and sure pages before this warp's
+    for (int r = 0; r < rank; ++r) {
+        tie_at += *cluster.map_shared_rank(&s_ties, r);
+        more_at += *cluster.map_shared_rank(&s_more, r);
+    }
+    if (C > 1) cluster_arrive_release();                         // done with the other CTAs' shared memory; waited for before leaving
+
+    // ---- second walk: every page to its place
+    const uint32_t below = (1u << lane) - 1u;
+    constexpr int kAhead = 4;                                    // groups whose table entries and weights are loaded together
+    for (int gr0 = g0; gr0 < g1; gr0 += kAhead) {
+        int32_t entry[kAhead];
+        float weight[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = (gr0 + k) * 32 + lane;
+            const bool in = gr0 + k < g1 && i < n;
+            entry[k] = in ? table[base + i] : 0;
+            weight[k] = in && ps == 1 ? w[base + i] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int gr = gr0 + k;
+            if (gr >= g1) break;
+            bool in, tie;
+            const bool above = classify(gr, &in, &tie);
+            const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie), sure_mask = __ballot_sync(0xffffffffu, above);
+            const bool stay = above || (tie && tie_at + __popc(tie_mask & below) < need);
+            const uint32_t stay_mask = __ballot_sync(0xffffffffu, stay);
+            const int i = base + gr * 32 + lane;
+            const int r = more_at + min(tie_at, need) + __popc(stay_mask & below);  // kept pages before this one
+            if (in) table_out[stay ? r : p.keep + i - r] = entry[k];
+            if (ps == 1) {
+                if (stay) w_out[r] = weight[k];
+            } else {
+                // the group's 32 pages end to end, four (or one) weights to a lane: independent loads, whatever the page size
+                const int first = (base + gr * 32) * ps, width = vec4 ? 4 : 1, steps = ps / width;
+#pragma unroll 4
+                for (int e = lane; e < 32 * steps; e += 32) {
+                    const int src = p.page_shift >= 0 ? e >> p.page_shift : e / steps, at = (e - src * steps) * width;
+                    const int to = __shfl_sync(0xffffffffu, r, src) * ps + at, from = first + src * ps + at;
+                    if (!(stay_mask >> src & 1u)) continue;
+                    if (width == 4 && from + 4 <= len) *reinterpret_cast<float4*>(w_out + to) = *reinterpret_cast<const float4*>(w + from);
+                    else
+                        for (int j = 0; j < width; ++j)
+                            if (from + j < len) w_out[to + j] = w[from + j];
+                }
             }
-            __syncthreads();
-            prefix |= s_digit << shift;
-            need = s_need;                                       // how many with exactly these leading digits stay
+            tie_at += __popc(tie_mask);
+            more_at += __popc(sure_mask);
         }
     }
-    int kept = 0, gone = 0, ties = 0;
-    for (int i0 = 0; i0 < used; i0 += nt) {
-        const int i = i0 + tid;
-        const bool in = i < used;
-        const bool competes = in && i >= lo && i < hi;
-        const uint32_t k = competes ? page_key(w, i, p.page_size, len) : 0u;
-        const bool any = p.keep > p.sink + p.recent;
-        const bool tie = competes && any && k == prefix;
-        int total;
-        const int tie_rank = ties + block_rank(tie, &total, warp_sums);
-        ties += total;
-        const bool stay = in && (!competes || (any && (k > prefix || (tie && tie_rank < need))));
-        const int r = kept + block_rank(stay, &total, warp_sums);
-        kept += total;
-        const int g = gone + block_rank(in && !stay, &total, warp_sums);
-        gone += total;
-        if (in) table_out[stay ? r : p.keep + g] = table[i];
-        if (stay) {
-            const int t0 = i * p.page_size, t1 = (int)min((int64_t)t0 + p.page_size, (int64_t)len);
-            for (int t = t0; t < t1; ++t) w_out[r * p.page_size + (t - t0)] = w[t];
-        }
-    }
-    const int new_len = len - (used - p.keep) * p.page_size;
-    for (int i = used + tid; i < max_pages; i += nt) table_out[i] = table[i];
-    for (int i = new_len + tid; i < len; i += nt) w_out[i] = 0.f;
-    for (int i = len + tid; i < p.max_len; i += nt) w_out[i] = w[i];
-    if (tid == 0) p.seq_lens_out[row] = new_len;
+    if (C > 1) cluster_wait();
 }
 
 }  // namespace tidal
@@ -188,8 +320,25 @@ extern "C" int tidal_evict_pages(const tidal_evict_args* a, void* stream) {
     TIDAL_REQUIRE((w + wb <= wo || wo + wb <= w) && (t + tb <= to || to + tb <= t) && (!l || l + lb <= lo || lo + lb <= l), TIDAL_ERR_ARG,
                   "evict_pages: outputs overlap the inputs");
     EvictParams p{a->d_weights, a->d_weights_out, a->weight_stride, a->d_page_table, a->d_page_table_out, a->page_table_stride,
-                  a->d_seq_lens, a->d_seq_lens_out, a->max_len, a->page_size, a->keep_pages, a->sink_pages, a->recent_pages};
-    TIDAL_CUDA_OK(launch_pdl(evict_pages_kernel, dim3(a->rows), dim3(1024), 0, (cudaStream_t)stream, 1, p));
+                  a->d_seq_lens, a->d_seq_lens_out, a->max_len, a->page_size, a->keep_pages, a->sink_pages, a->recent_pages, 0, 0, 0, 0, -1};
+    p.row_vec4 = a->weight_stride % 4 == 0 && (((uintptr_t)a->d_weights | (uintptr_t)a->d_weights_out) & 15) == 0;
+    p.table_vec4 = a->page_table_stride % 4 == 0 && (((uintptr_t)a->d_page_table | (uintptr_t)a->d_page_table_out) & 15) == 0;
+    p.vec4 = p.row_vec4 && a->page_size % 4 == 0;
+    const int steps = p.vec4 ? a->page_size / 4 : a->page_size;
+    if ((steps & (steps - 1)) == 0) p.page_shift = 31 - __builtin_clz((unsigned)steps);
+    // CTAs per row: one CTA takes 1.3 us for every 1024 pages and as much for 4096 weights of longer pages; a second, the
+    // fourth and the eighth each add 2 us or more of barriers.  Measured, in us, with 1 / 2 / 4 / 8 CTAs: 4096 single-token
+    // pages 10.1 / 10.8 / 11.7 / 14.5, 16 K 22.5 / 16.7 / 14.5 / 16.5, 128 K 177 / 96 / 43 / 31, 8192 pages of 16 tokens
+    // 37 / 25 / 19 / 20.  Clusters beyond one to an SM would wait for each other (32 rows of 32 K: 19 with 4, 55 with 8).
+    const int64_t load = max_pages + (a->page_size > 1 ? a->max_len / 4 : 0);
+    int C = load < 6144 ? 1 : load < 12288 ? 2 : load < 45056 ? 4 : 8;
+    while (C > 1 && (int64_t)a->rows * C > sm_count_cached()) C /= 2;
+    TIDAL_REQUIRE((int64_t)a->rows * C <= INT32_MAX, TIDAL_ERR_ARG, "evict_pages: too many rows");
+    const int64_t per_cta = ((max_pages + 31) / 32 + C - 1) / C * 32;
+    const size_t smem = sizeof(uint32_t) * (size_t)(per_cta <= kEvictKeys ? per_cta : 0);
+    p.cached = smem > 0;
+    if (smem > 16384) TIDAL_CUDA_OK(cudaFuncSetAttribute(evict_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictKeys * 4));
+    TIDAL_CUDA_OK(launch_pdl(evict_pages_kernel, dim3(a->rows * C), dim3(kEvictThreads), smem, (cudaStream_t)stream, C, p));
     count_launch();
     return TIDAL_OK;
 }
