@@ -528,7 +528,7 @@ typedef struct {
     const float* d_lse;          /* [batch][heads] */
     float* d_weights;            /* [batch][weight_stride], updated in place */
     int64_t weight_stride;
-    const int32_t* d_seq_lens;   /* [batch] or NULL: all = seq_len */
+    const int32_t* d_seq_lens;   /* [batch], batch <= 1024, or NULL: all = seq_len */
     int32_t seq_len;             /* upper bound of (and default for) the lengths */
     int32_t batch, heads;
     float decay;

@@ -95,7 +95,7 @@ def test_attention_needs_an_initialised_workspace(L):
 WEIGHTS = dict(d_scores=256, score_stride=100, d_lse=256, d_weights=256, weight_stride=100, seq_len=100, batch=1, heads=8, decay=1.0)
 
 
-@pytest.mark.parametrize("change,match", [(dict(d_lse=0), "must be given"), (dict(batch=0), "batch"), (dict(heads=0), "heads"), (dict(seq_len=101), "shorter"),
+@pytest.mark.parametrize("change,match", [(dict(d_lse=0), "must be given"), (dict(batch=0), "batch"), (dict(heads=0), "heads"), (dict(batch=1025, d_seq_lens=256), "1024"), (dict(seq_len=101), "shorter"),
                                           (dict(weight_stride=99), "shorter"), (dict(seq_len=-1), "shorter")])
 def test_weights_refusals(L, change, match):
     _refused(L, "tidal_accumulate_weights", _fill(L.WeightsArgs(), **{**WEIGHTS, **change}), None, match=match)
