@@ -16,7 +16,7 @@ struct WeightsParams {
     float* weights;
     int64_t weight_stride;
     const int32_t* seq_lens;
-    int32_t seq_len, heads, head_warps, batch, steps;
+    int32_t seq_len, heads, batch, strips, warps;     // strips of seq_len tokens; warps that fill the device
     float decay;
 };
 
@@ -54,40 +54,48 @@ __global__ void __launch_bounds__(256, 4) accumulate_weights_kernel(const Weight
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int strips = 8 / p.head_warps, strip = warp / p.head_warps, h0 = warp - strip * p.head_warps;
-    const int tokens = strips * kWeightTokens;                   // a CTA's tokens per step
-    auto steps_of = [&](int i) -> int {
+    auto strips_of = [&](int i) -> int {
         const int n = i < p.batch ? min(p.seq_lens[i], p.seq_len) : 0;
-        return n > 0 ? (n - 1) / tokens + 1 : 0;
+        return n > 0 ? (n - 1) / kWeightTokens + 1 : 0;
     };
-    int64_t total;
+    int64_t total;                                               // strips of all sequences
     if (p.seq_lens) {
         int own = 0;
         const int first = threadIdx.x * (kWeightBatch / 256);
-        for (int i = 0; i < kWeightBatch / 256; ++i) own += steps_of(first + i);
+        for (int i = 0; i < kWeightBatch / 256; ++i) own += strips_of(first + i);
         int at = block_inclusive(own, scan) - own;
         for (int i = 0; i < kWeightBatch / 256; ++i) {
             before[first + i] = at;
-            at += steps_of(first + i);
+            at += strips_of(first + i);
         }
         if (threadIdx.x == 255) before[kWeightBatch] = at;
         __syncthreads();
         total = before[kWeightBatch];
     } else {
-        total = (int64_t)p.batch * p.steps;
+        total = (int64_t)p.batch * p.strips;
     }
-    int b = 0;
-    for (int64_t step = blockIdx.x; step < total; step += gridDim.x) {
-        int64_t cta0;
+    // warps per strip: as many as heads (up to 8) while there are few strips, one (no barrier) when the strips alone fill the
+    // SMs (8 sequences of 128 K tokens, 32 heads: 40 us with 8 warps to a strip, 25 with one)
+    int hw = p.heads >= 8 ? 8 : p.heads >= 4 ? 4 : p.heads >= 2 ? 2 : 1;
+    while (hw > 1 && total * hw > p.warps) hw >>= 1;
+    const int per_cta = 8 / hw, h0 = warp % hw;
+    for (int64_t step = blockIdx.x; step * per_cta < total; step += gridDim.x) {
+        const int64_t q = step * per_cta + warp / hw;            // this warp's strip
+        int b = 0, strip = 0;
         if (p.seq_lens) {
-            while (before[b + 1] <= step) ++b;
-            cta0 = (step - before[b]) * tokens;
-        } else {
-            b = (int)(step / p.steps);
-            cta0 = (step - (int64_t)b * p.steps) * tokens;
+            int hi = kWeightBatch;                               // last sequence that starts at or before the strip
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (before[mid] <= q) b = mid; else hi = mid;
+            }
+            strip = (int)(q - before[b]);
+        } else if (q < total) {
+            b = (int)(q / p.strips);
+            strip = (int)(q - (int64_t)b * p.strips);
         }
-        const int len = p.seq_lens ? min(p.seq_lens[b], p.seq_len) : p.seq_len;
-        const int64_t j0 = cta0 + strip * kWeightTokens;             // token of lane 0
+        const int len = q >= total ? 0 : p.seq_lens ? min(p.seq_lens[b], p.seq_len) : p.seq_len;
+        if (q >= total) b = 0, strip = 0;
+        const int64_t j0 = (int64_t)strip * kWeightTokens;       // token of lane 0
         const float* s = p.scores + (size_t)b * p.heads * p.score_stride + j0;
         const float* z = p.lse + (size_t)b * p.heads;
         float acc[4] = {};
@@ -96,20 +104,20 @@ __global__ void __launch_bounds__(256, 4) accumulate_weights_kernel(const Weight
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] += fast_exp2((x[i] - zh) * kLog2e);
         };
-        const size_t stride = (size_t)p.head_warps * p.score_stride;
+        const size_t stride = (size_t)hw * p.score_stride;
         const float* row = s + (size_t)h0 * p.score_stride;
         if (VEC && j0 + kWeightTokens <= len) {
             const float* at = row + 4 * lane;
             int h = h0;
             auto batch = [&](auto count) {                       // as many heads as their loads are in flight together
                 constexpr int K = decltype(count)::value;
-                for (; h + (K - 1) * p.head_warps < p.heads; h += K * p.head_warps, at += K * stride) {
+                for (; h + (K - 1) * hw < p.heads; h += K * hw, at += K * stride) {
                     float4 v[K];
                     float zh[K];
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
                         v[k] = __ldcs(reinterpret_cast<const float4*>(at + k * stride));
-                        zh[k] = z[h + k * p.head_warps];
+                        zh[k] = z[h + k * hw];
                     }
 #pragma unroll
                     for (int k = 0; k < K; ++k) add({v[k].x, v[k].y, v[k].z, v[k].w}, zh[k]);
@@ -119,7 +127,7 @@ __global__ void __launch_bounds__(256, 4) accumulate_weights_kernel(const Weight
             batch(std::integral_constant<int, 4>());
             batch(std::integral_constant<int, 1>());
         } else if (j0 < len) {
-            for (int h = h0; h < p.heads; h += p.head_warps, row += stride) {
+            for (int h = h0; h < p.heads; h += hw, row += stride) {
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -129,8 +137,8 @@ __global__ void __launch_bounds__(256, 4) accumulate_weights_kernel(const Weight
                 add(x, z[h]);
             }
         }
-        if (p.head_warps == 1) {                                 // the warp has its tokens' sums: no other warp is waited for
-            float* w = p.weights + (size_t)b * p.weight_stride + j0;
+        float* w = p.weights + (size_t)b * p.weight_stride + j0;
+        if (hw == 1) {                                           // the warp has its tokens' sums: no other warp is waited for
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = VEC ? 4 * lane + i : lane + 32 * i;
@@ -141,11 +149,10 @@ __global__ void __launch_bounds__(256, 4) accumulate_weights_kernel(const Weight
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[warp][VEC ? 4 * lane + i : lane + 32 * i] = acc[i];
         __syncthreads();
-        for (int t = threadIdx.x; t < tokens && cta0 + t < len; t += 256) {
+        for (int t = h0 * 32 + lane; t < kWeightTokens && j0 + t < len; t += 32 * hw) {
             float sum = 0.f;
-            for (int k = 0; k < p.head_warps; ++k) sum += sums[t / kWeightTokens * p.head_warps + k][t % kWeightTokens];
-            float* w = p.weights + (size_t)b * p.weight_stride + cta0 + t;
-            *w = p.decay * *w + sum;
+            for (int k = 0; k < hw; ++k) sum += sums[warp - h0 + k][t];
+            w[t] = p.decay * w[t] + sum;
         }
         __syncthreads();
     }
@@ -389,15 +396,10 @@ extern "C" int tidal_accumulate_weights(const tidal_weights_args* a, void* strea
     TIDAL_REQUIRE(a->seq_len >= 0 && a->score_stride >= a->seq_len && a->weight_stride >= a->seq_len, TIDAL_ERR_ARG,
                   "accumulate_weights: rows of scores or weights shorter than seq_len %d", a->seq_len);
     if (a->seq_len == 0) return TIDAL_OK;
-    // Warps per strip: as many as heads (up to 8) while there are few strips, one (no barrier) when the strips alone fill the
-    // SMs.  8 sequences of 128 K tokens, 32 heads: 40 us with 8 warps to a strip.
-    int hw = a->heads >= 8 ? 8 : a->heads >= 4 ? 4 : a->heads >= 2 ? 2 : 1;
-    const int64_t strips = (a->seq_len + (int64_t)kWeightTokens - 1) / kWeightTokens * a->batch;
-    while (hw > 1 && strips * hw > (int64_t)24 * sm_count_cached()) hw /= 2;
-    const int tokens = 8 / hw * kWeightTokens;
-    const int steps = (int)((a->seq_len + (int64_t)tokens - 1) / tokens);
-    const WeightsParams p{a->d_scores, a->score_stride, a->d_lse, a->d_weights, a->weight_stride, a->d_seq_lens, a->seq_len, a->heads, hw, a->batch, steps, a->decay};
-    const dim3 grid((unsigned)std::min<int64_t>((int64_t)a->batch * steps, 8 * sm_count_cached()));
+    const int strips = (int)((a->seq_len + (int64_t)kWeightTokens - 1) / kWeightTokens);
+    const WeightsParams p{a->d_scores, a->score_stride, a->d_lse, a->d_weights, a->weight_stride, a->d_seq_lens, a->seq_len, a->heads, a->batch, strips,
+                          40 * sm_count_cached(), a->decay};
+    const dim3 grid((unsigned)std::min<int64_t>((int64_t)a->batch * strips, 4 * sm_count_cached()));
     const bool vec = a->score_stride % 4 == 0 && ((uintptr_t)a->d_scores & 15) == 0;
     if (vec) TIDAL_CUDA_OK(launch_pdl(accumulate_weights_kernel<true>, grid, dim3(256), 0, (cudaStream_t)stream, 1, p));
     else TIDAL_CUDA_OK(launch_pdl(accumulate_weights_kernel<false>, grid, dim3(256), 0, (cudaStream_t)stream, 1, p));
