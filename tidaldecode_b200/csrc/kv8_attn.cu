@@ -38,7 +38,9 @@ namespace tidal {
 
 constexpr int kKv8Warps = 8;
 constexpr int kKv8Tile = 16;             // tokens a warp takes at a time; it looks them up two tiles at a time
-constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself; beyond, a CTA per list
+constexpr int kKv8SoloTokens = 1024;     // lists up to this long go to a CTA each
 
 struct AttnKv8Params {
     const void* q;
@@ -55,17 +57,18 @@ struct AttnKv8Params {
     float* scores;
     int64_t score_stride;
     float* lse;
-    float* part_o;               // [slices][ctas + lists][HC * rows][D]
-    float* part_ml;              // [slices][ctas + lists][HC * rows][2]
-    uint32_t* arrivals;          // [lists * slices][16], zero at rest
+    float* part_o;               // [units][ranges + lists][rows][D]: what a warp has of a list that it shares with others
+    float* part_ml;              // [units][ranges + lists][rows][2]
+    int32_t* part_prefix;        // [lists + 1] pairs of tiles before each list, for the merge (ragged)
     uint32_t* status;
     int32_t Hq, Hkv, G, block;
     int32_t lists, per_head;     // token lists: one per sequence, or one per (sequence, query head)
-    int32_t groups, rows;        // query heads of a KV head are taken `rows` (at most 16) at a time, in `groups` groups
-    int32_t HC, slices;          // (KV head, group) units per CTA; CTAs along the units
-    int32_t ctas;                // CTAs that share the lists' tiles
-    int32_t ragged;              // lengths differ: 1 = they are added up by every CTA, 2 = a CTA per list
-    int32_t tiles_per_list;      // ragged == 0
+    int32_t groups, rows, units; // query heads of a KV head are taken `rows` (at most 16) at a time, in `groups` groups: a unit each
+    int32_t HC, slices;          // units per CTA (its warps take them in turn); CTAs along the units
+    int32_t ctas, ranges;        // CTAs that share the lists' tokens; ranges of them per unit: ctas * warps / HC
+    int32_t solo;                // a CTA per list (and unit): its warps split the list and merge in shared memory
+    int32_t ragged;              // lengths are on the device; every CTA adds them up
+    int32_t pairs_per_list;      // !ragged
     int32_t page_shift, block_shift;     // -1 where the size is no power of two
     int32_t blocks_per_page;
     float sm_scale;
@@ -112,9 +115,10 @@ __device__ __forceinline__ int list_len_kv8(const AttnKv8Params& p, int list) {
     return p.seq_lens ? max(0, min(p.seq_lens[list], p.seq_len)) : p.seq_len;
 }
 
-template <int D>
+// More than 8 query heads to a unit at D = 128 take all registers of an SM for one CTA; its ring then takes the whole memory.
+template <int D, bool R2>
 struct Kv8Ring {
-    static constexpr int stages = D == 128 ? 3 : 5;
+    static constexpr int stages = D == 128 ? (R2 ? 6 : 3) : 5;
     static constexpr int stage_bytes = kKv8Tile * 2 * D;                 // of one warp: K rows, then V rows
     static constexpr size_t bytes = (size_t)kKv8Warps * stages * stage_bytes;
 };
@@ -151,249 +155,277 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
+// Softmax statistics and output of one query head to their final form.
+__device__ __forceinline__ float attn_kv8_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
+// Which of `ranges` equal ranges of `total` items holds item i, and where range r begins.  ranges <= total.
+__device__ __forceinline__ int range_begin(int r, int total, int ranges) { return (int)((int64_t)r * total / ranges); }
+__device__ __forceinline__ int range_of(int i, int total, int ranges) { return (int)((((int64_t)i + 1) * ranges - 1) / total); }
+
+// Work is dealt out in pairs of tiles, 32 tokens.  Laid end to end, the pairs of all token lists are cut into equal ranges, one
+// to a warp and unit (KV head, or up to 16 query heads of one), whatever list they fall into: a batch of very different
+// lengths keeps every SM busy to the end.  A warp keeps its ring full across the lists' borders and waits for no other
+// warp; where a list is shared, each leaves a partial (o relative to m, m, l) and merge_kv8_kernel adds them in order.
+// The order of additions depends on the lengths and the launch alone.  Short lists go the other way (solo): one CTA per
+// list and unit, whose warps merge through shared memory, with no second launch.
 template <typename T, int D, bool R2>    // R2: more than 8 query heads to a unit
-__global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
+__global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 128) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
     constexpr bool QS = sizeof(T) == 4, PS = !std::is_same<T, __nv_bfloat16>::value;
-    constexpr int S = Kv8Ring<D>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
+    constexpr int S = Kv8Ring<D, R2>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int NP = S <= 4 ? 2 : 4;       // pairs of tiles whose scales are kept: a slot is refilled S - 2 NP <= 0 tiles after its last use
     // per token: scale of K (-1: no token) and exponent of the scale of V (-inf: the block reads as zeros)
     __shared__ __align__(16) float2 sc_ring[kKv8Warps][NP][2 * kKv8Tile];
     __shared__ float ml[kKv8Warps][16][2];
-    __shared__ int s_scan[kKv8Warps + 1];
-    __shared__ int s_last;
-    int* prefix = reinterpret_cast<int*>(smem + Kv8Ring<D>::bytes);    // [lists + 1] when the lengths are added up here
+    __shared__ int s_scan[kKv8Warps];
+    int* prefix = reinterpret_cast<int*>(smem + Kv8Ring<D, R2>::bytes);      // [lists + 1] when the lengths are added up here
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int TG = kKv8Warps / p.HC, TT = 2 * kKv8Tile * TG;
-    const int uw = warp % p.HC, tg = warp / p.HC;
-    const int cta = blockIdx.y, slice = blockIdx.x;
-    unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D>::stage_bytes;
-
+    const int TG = kKv8Warps / p.HC, uw = warp % p.HC, tg = warp / p.HC;
+    const int cta = (int)(blockIdx.x / (uint32_t)p.slices), slice = (int)(blockIdx.x - (uint32_t)cta * (uint32_t)p.slices);
+    unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D, R2>::stage_bytes;
+    constexpr int PAIR = 2 * kKv8Tile;
     if (tid == 0) TIDAL_STAMP(0);
     pdl_wait();
     pdl_launch_dependents();
     if (tid == 0) TIDAL_STAMP(1);
 
-    // ---- this CTA's range of tiles
-    int64_t tile, tile_end;
-    int total;
-    if (p.ragged == 0) {
-        total = p.tiles_per_list * p.lists;
-    } else if (p.ragged == 1) {
-        const int per = (p.lists + blockDim.x - 1) / blockDim.x, first = tid * per;
-        int sum = 0;
-        for (int i = first; i < min(first + per, p.lists); ++i) sum += max(1, (list_len_kv8(p, i) + TT - 1) / TT);
-        int incl = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += y;
-        }
-        if (lane == 31) s_scan[warp] = incl;
-        __syncthreads();
-        int at = incl - sum;
-        for (int i = 0; i < warp; ++i) at += s_scan[i];
-        for (int i = first; i < min(first + per, p.lists); ++i) {
-            prefix[i] = at;
-            at += max(1, (list_len_kv8(p, i) + TT - 1) / TT);
-            if (i == p.lists - 1) prefix[p.lists] = at;
-        }
-        __syncthreads();
-        total = prefix[p.lists];
-    } else {
-        total = p.lists;
-    }
-    const int ctas = min(p.ctas, total);                                 // no CTA without a tile: every part that is waited for comes
-    if (cta >= ctas) return;
-    auto cta_begin = [&](int c) -> int { return (int)((int64_t)c * total / ctas); };
-    auto cta_of = [&](int tl) -> int { return (int)((((int64_t)tl + 1) * ctas - 1) / total); };       // the CTA whose range holds the tile
-    tile = p.ragged == 2 ? cta : cta_begin(cta);
-    tile_end = p.ragged == 2 ? cta + 1 : cta_begin(cta + 1);
-    int list = 0;
-    if (p.ragged == 0) {
-        list = tile < total ? (int)(tile / p.tiles_per_list) : 0;
-    } else if (p.ragged == 1) {
-        int lo = 0, hi = p.lists;                                        // last list that starts at or before the tile
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (prefix[mid] <= tile) lo = mid; else hi = mid;
-        }
-        list = lo;
-    } else {
+    // ---- this warp's range [t0, t1) of pairs
+    auto pairs_of = [&](int len) -> int { return len > 0 ? (len - 1) / PAIR + 1 : 1; };     // an empty list has one empty pair
+    int t0, t1, list = 0, first = 0;                                     // `list` starts at pair `first`
+    if (p.solo) {
         list = cta;
+        const int n = pairs_of(list_len_kv8(p, list));
+        t0 = range_begin(tg, n, TG);
+        t1 = range_begin(tg + 1, n, TG);
+    } else {
+        int total;
+        if (p.ragged) {
+            const int per = (p.lists + blockDim.x - 1) / blockDim.x, own0 = tid * per;
+            int sum = 0;
+            for (int i = own0; i < min(own0 + per, p.lists); ++i) sum += pairs_of(list_len_kv8(p, i));
+            int incl = sum;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += y;
+            }
+            if (lane == 31) s_scan[warp] = incl;
+            __syncthreads();
+            int at = incl - sum;
+            for (int i = 0; i < warp; ++i) at += s_scan[i];
+            for (int i = own0; i < min(own0 + per, p.lists); ++i) {
+                prefix[i] = at;
+                at += pairs_of(list_len_kv8(p, i));
+                if (i == p.lists - 1) prefix[p.lists] = at;
+            }
+            __syncthreads();
+            total = prefix[p.lists];
+            if (cta == 0 && slice == 0)
+                for (int i = tid; i <= p.lists; i += blockDim.x) p.part_prefix[i] = prefix[i];
+        } else {
+            total = p.pairs_per_list * p.lists;
+        }
+        const int ranges = min(p.ranges, total), r = cta * TG + tg;      // no range without a pair: every part that is added exists
+        if (r >= ranges) return;
+        t0 = range_begin(r, total, ranges);
+        t1 = range_begin(r + 1, total, ranges);
+        if (p.ragged) {
+            int hi = p.lists;                                            // last list that starts at or before t0
+            while (hi - list > 1) {
+                const int mid = (list + hi) >> 1;
+                if (prefix[mid] <= t0) list = mid; else hi = mid;
+            }
+            first = prefix[list];
+        } else {
+            list = t0 / p.pairs_per_list;
+            first = list * p.pairs_per_list;
+        }
     }
+    const int unit = slice * p.HC + uw;
 
-    for (; tile < tile_end; ++list) {
-        // ---- the segment of `list` that lies in this CTA's range: entries [tok0, tok1)
-        const int len = list_len_kv8(p, list);
-        int first_tile, n_tiles;
-        if (p.ragged == 0) first_tile = list * p.tiles_per_list, n_tiles = p.tiles_per_list;
-        else if (p.ragged == 1) first_tile = prefix[list], n_tiles = prefix[list + 1] - first_tile;
-        else first_tile = list, n_tiles = 1;
-        const int seg_end = (int)min(tile_end, (int64_t)first_tile + n_tiles);
-        const bool whole = p.ragged == 2 || (tile == first_tile && seg_end == first_tile + n_tiles);
-        const int tok0 = p.ragged == 2 ? 0 : (int)min((int64_t)len, (tile - first_tile) * TT);
-        const int tok1 = p.ragged == 2 ? len : (int)min((int64_t)len, (int64_t)(seg_end - first_tile) * TT);
-        const int w0 = tok0 + tg * 2 * kKv8Tile;                         // first token of this warp; it takes 32 of every TT
-        const int n_pairs = tok1 > w0 ? (tok1 - w0 + TT - 1) / TT : 0;
-        int n_it = 2 * n_pairs;                                          // its tiles (an empty one at the end is left out)
-        if (n_pairs > 0 && w0 + (n_pairs - 1) * TT + kKv8Tile >= tok1) --n_it;
+    // ---- where a list's tokens and heads are
+    struct List {
+        int list, first, next;           // pairs [first, next)
+    };
+    auto enter = [&](List& w, int i, int at) -> int {
+        const int len = list_len_kv8(p, i);
+        w.list = i;
+        w.first = at;
+        w.next = at + pairs_of(len);
+        return len;
+    };
+    const int unit_kvh = unit / p.groups, unit_hq = unit_kvh * p.G + (unit - unit_kvh * p.groups) * p.rows;
+    auto seq_of = [&](int i) -> int { return p.per_head ? i / p.Hq : i; };                          // sequence of a list
+    auto kvh_of = [&](int i) -> int { return p.per_head ? i % p.Hq / p.G : unit_kvh; };
+    auto row_of = [&](int i) -> size_t { return p.per_head ? (size_t)i : (size_t)i * p.Hq + unit_hq; };     // row of its first query head
+    const int heads = p.per_head ? 1 : min(p.rows, (unit_kvh + 1) * p.G - unit_hq);                // query heads of the unit
 
-        const int b = p.per_head ? list / p.Hq : list;
-        const int unit = slice * p.HC + uw;
-        const int kvh = p.per_head ? (list - b * p.Hq) / p.G : unit / p.groups;
-        const int hq0 = p.per_head ? list - b * p.Hq : kvh * p.G + (unit - kvh * p.groups) * p.rows;
-        const int heads = p.per_head ? 1 : min(p.rows, (kvh + 1) * p.G - hq0);         // query heads of this unit
-        const int seq = p.seq_lens ? max(0, min(p.seq_lens[b], p.seq_len)) : p.seq_len;
-
-        // ---- Q fragments (lane: head g of each eight), scaled to [2^11, 2^12) per head
-        uint32_t qa[NR][KS][2], ql[QS ? NR : 1][QS ? KS : 1][2];
-        float qn[NR][2], qn2[NR][2];                                     // of heads 2t, 2t+1: undo the scaling and apply sm_scale (qn2 in log2 units)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int head = g + 8 * r;
-            const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)b * p.Hq + hq0 + (head < heads ? head : 0)) * D;
-            float f[KS][4], top = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                load4(qrow + (ks >> 2) * 64 + t * 16 + (ks & 3) * 4, f[ks]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = fabsf(f[ks][i]);
-                    top = a < INFINITY ? fmaxf(top, a) : top;
-                }
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            int sh = 138 - (int)(__float_as_uint(top) >> 23);           // 11 less the exponent of the largest element
-            sh = top == 0.f ? 0 : min(sh, 120);
-            const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-            const float down = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                qn[r][e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
-                qn2[r][e] = qn[r][e] * kLog2e;
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float x0 = f[ks][2 * i] * up, x1 = f[ks][2 * i + 1] * up;
-                    qa[r][ks][i] = head < heads ? pack_f16(x0, x1) : 0u;
-                    if (QS) ql[QS ? r : 0][QS ? ks : 0][i] = head < heads ? pack_f16_rest(x0, x1, qa[r][ks][i]) : 0u;
-                }
+    // ---- looking tokens up: lane i follows token i of a pair; its list entry is loaded two pairs ahead of its copies, its
+    //      page one pair ahead, its scales with the copies
+    constexpr int PR = D / 16, TI = 32 / PR;                              // 16-byte pieces of a row; tokens that one copy of the warp covers
+    const int c_tok = lane / PR, c_piece = lane % PR;
+    const int ps = p.map.page_size;
+    const uint32_t pitch = (uint32_t)p.Hkv * D;
+    const uint32_t ring_k = smem_u32(ring) + k_piece<D>(c_tok, c_piece), ring_v = smem_u32(ring) + kKv8Tile * D + v_piece<D>(c_tok, c_piece);
+    const int k_off = k_piece<D>(g, t), v_off = v_piece<D>(2 * t, g * VB / 16) + (g * VB & 15);
+    const int v_off1 = v_piece<D>(2 * t + 1, g * VB / 16) + (g * VB & 15);
+    const uint32_t sc_plane = (uint32_t)p.blocks_per_page * p.Hkv;
+    List ahead_l;                                                        // of the pair whose entries are loaded next
+    int ahead_t = t0, ahead_len = enter(ahead_l, list, first);
+    auto fetch_pos = [&]() -> int {
+        const int i = (ahead_t - ahead_l.first) * PAIR + lane;
+        if (ahead_t >= t1 || i >= ahead_len) return INT_MIN;             // no token here
+        return p.sel_idx ? max(p.sel_idx[(size_t)ahead_l.list * p.sel_stride + i], -1) : i;
+    };
+    auto step_ahead = [&]() {
+        ++ahead_t;
+        if (ahead_t == ahead_l.next && ahead_t < t1) ahead_len = enter(ahead_l, ahead_l.list + 1, ahead_t);
+    };
+    auto page_of = [&](int pos) -> int { return p.page_shift >= 0 ? pos >> p.page_shift : pos / ps; };
+    auto fetch_page = [&](int pos, int i) -> int {
+        const int b = seq_of(i);
+        if (p.sel_idx && pos >= (p.seq_lens ? min(p.seq_lens[b], p.seq_len) : p.seq_len)) return -1;
+        if (pos < 0) return -1;
+        return p.map.page_table ? p.map.page_table[(size_t)b * p.map.pt_stride + page_of(pos)] : (int)((int64_t)b * p.map.pt_stride) + page_of(pos);
+    };
+    int list_c = ahead_l.list, pos_c = fetch_pos(), page_c = fetch_page(pos_c, list_c);            // the pair to be copied next
+    step_ahead();
+    int list_n = ahead_l.list, pos_n = fetch_pos();                                                // the one behind it
+    step_ahead();
+    int row = -1;                                                        // pool row of the lane's K row (its V row lies ps rows further), or -1
+    uint32_t sc_k = 0, sc_v = 0;                                         // its scale bytes
+    uint32_t head_off = 0;                                               // byte offset of its head (and the lane's piece) in a row
+    uint32_t full = 0, half = 0;     // bit i, of the pair copied i pairs ago: every token is there; a token of its second tile is there
+    auto look_up = [&]() {
+        row = -1;
+        const uint32_t kvh = (uint32_t)kvh_of(list_c);
+        if (page_c >= 0 && page_c < (int)p.map.num_pages) {
+            const int entry = pos_c - page_of(pos_c) * ps;
+            row = page_c * 2 * ps + entry;
+            uint32_t at = (uint32_t)page_c * 2u * sc_plane + kvh;              // scale bytes number less than 2^32, checked on the host
+            if (p.blocks_per_page > 1) at += (uint32_t)(p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block) * (uint32_t)p.Hkv;
+            sc_k = p.scales[at];
+            sc_v = p.scales[at + sc_plane];
+        } else if (pos_c != INT_MIN) {
+            atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
         }
-
-        float o[NR][KS][4];                                              // [eight heads][16 elements]: elements 2j, 2j+1 of g*D/8.., heads 2t, 2t+1
-        float m[NR][2], M[NR][2], l[NR][2];
+        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+        full = full << 1 | (there == 0xffffffffu ? 1u : 0u);
+        half = half << 1 | (there >> kKv8Tile ? 1u : 0u);
+        head_off = kvh * D + c_piece * 16;
+        page_c = fetch_page(pos_n, list_n);
+        pos_c = pos_n;
+        list_c = list_n;
+        pos_n = fetch_pos();
+        list_n = ahead_l.list;
+        step_ahead();
+    };
+    auto park_scales = [&](int pair) {
+        sc_ring[warp][pair & (NP - 1)][lane] = row >= 0 ? make_float2(scale_value(sc_k), sc_v ? (float)((int)sc_v - 127) : -INFINITY) : make_float2(-1.f, -INFINITY);
+    };
+    auto copy = [&](int it, uint32_t slot) {
+        if ((it & 1) && !(half & 1u)) return;
+        const int l0 = (it & 1) * kKv8Tile + c_tok;
+        const uint8_t *k_src = p.kv + head_off, *v_src = k_src + (size_t)ps * pitch;
+        if (full & 1u) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                m[r][e] = M[r][e] = -FLT_MAX;
-                l[r][e] = 0.f;
+            for (int i = 0; i < kKv8Tile / TI; ++i) {
+                const uint32_t r = (uint32_t)__shfl_sync(0xffffffffu, row, l0 + i * TI);
+                cp_async16(ring_k + slot + i * 512, k_src + (uint64_t)r * pitch);
+                cp_async16((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + (uint64_t)r * pitch);
             }
+        } else {
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[r][j][i] = 0.f;
+            for (int i = 0; i < kKv8Tile / TI; ++i) {
+                const int r = __shfl_sync(0xffffffffu, row, l0 + i * TI);
+                const uint64_t at = (uint64_t)max(r, 0) * pitch;
+                cp_async16_or_zero(ring_k + slot + i * 512, k_src + at, r >= 0);
+                cp_async16_or_zero((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + at, r >= 0);
+            }
         }
+    };
 
-        // ---- looking tokens up: lane i follows token i of a pair of tiles; its list entry is loaded two pairs ahead of
-        //      its copies, its page one pair ahead, its scales with the copies
-        constexpr int PR = D / 16, TI = 32 / PR;                          // 16-byte pieces of a row; tokens that one copy of the warp covers
-        const int c_tok = lane / PR, c_piece = lane % PR;
-        const int ps = p.map.page_size;
-        const uint32_t pitch = (uint32_t)p.Hkv * D;
-        const uint8_t* k_src = p.kv + (size_t)kvh * D + c_piece * 16;
-        const uint8_t* v_src = k_src + (size_t)ps * pitch;
-        const uint32_t ring_k = smem_u32(ring) + k_piece<D>(c_tok, c_piece), ring_v = smem_u32(ring) + kKv8Tile * D + v_piece<D>(c_tok, c_piece);
-        const int k_off = k_piece<D>(g, t), v_off = v_piece<D>(2 * t, g * VB / 16) + (g * VB & 15);
-        const int v_off1 = v_piece<D>(2 * t + 1, g * VB / 16) + (g * VB & 15);
-        const int32_t* sel = p.sel_idx ? p.sel_idx + (size_t)list * p.sel_stride : nullptr;
-        const int32_t* table = p.map.page_table ? p.map.page_table + (size_t)b * p.map.pt_stride : nullptr;
-        const int page0 = (int)((int64_t)b * p.map.pt_stride);           // without a table
-        const uint8_t* sc_src = p.scales + kvh;
-        const uint32_t sc_plane = (uint32_t)p.blocks_per_page * p.Hkv;
-        auto fetch_pos = [&](int pair) -> int {
-            const int i = w0 + pair * TT + lane;
-            if (pair >= n_pairs || i >= tok1) return INT_MIN;            // no token here
-            return sel ? max(sel[i], -1) : i;
-        };
-        auto page_of = [&](int pos) -> int { return p.page_shift >= 0 ? pos >> p.page_shift : pos / ps; };
-        auto fetch_page = [&](int pos) -> int {
-            if (pos < 0 || pos >= seq) return -1;
-            return table ? table[page_of(pos)] : page0 + page_of(pos);
-        };
-        int pos_c = fetch_pos(0), page_c = fetch_page(pos_c), pos_n = fetch_pos(1);
-        int row = -1;                                                    // pool row of the lane's K row (its V row lies ps rows further), or -1
-        uint32_t sc_k = 0, sc_v = 0;                                     // its scale bytes
-        uint32_t full = 0;                                               // bit i: every token of the pair issued i pairs ago is there
-        auto look_up = [&](int pair) {
-            row = -1;
-            if (page_c >= 0 && page_c < (int)p.map.num_pages) {
-                const int entry = pos_c - page_of(pos_c) * ps;
-                row = page_c * 2 * ps + entry;
-                uint32_t at = (uint32_t)page_c * 2u * sc_plane;          // scale bytes number less than 2^32, checked on the host
-                if (p.blocks_per_page > 1) at += (uint32_t)(p.block_shift >= 0 ? entry >> p.block_shift : entry / p.block) * (uint32_t)p.Hkv;
-                sc_k = sc_src[at];
-                sc_v = sc_src[at + sc_plane];
-            } else if (pos_c != INT_MIN) {
-                atomicOr(p.status, TIDAL_DEV_BAD_INDEX);
-            }
-            full = full << 1 | (__all_sync(0xffffffffu, row >= 0) ? 1u : 0u);
-            page_c = fetch_page(pos_n);
-            pos_c = pos_n;
-            pos_n = fetch_pos(pair + 2);
-        };
-        auto park_scales = [&](int pair) {
-            sc_ring[warp][pair & (NP - 1)][lane] = row >= 0 ? make_float2(scale_value(sc_k), sc_v ? (float)((int)sc_v - 127) : -INFINITY) : make_float2(-1.f, -INFINITY);
-        };
-        auto copy = [&](int it, uint32_t slot) {
-            const int l0 = (it & 1) * kKv8Tile + c_tok;
-            if (full & 1u) {
+    const int n_it = 2 * (t1 - t0);                                      // tiles (the second of a pair may be empty)
 #pragma unroll
-                for (int i = 0; i < kKv8Tile / TI; ++i) {
-                    const uint32_t r = (uint32_t)__shfl_sync(0xffffffffu, row, l0 + i * TI);
-                    cp_async16(ring_k + slot + i * 512, k_src + (uint64_t)r * pitch);
-                    cp_async16((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + (uint64_t)r * pitch);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kKv8Tile / TI; ++i) {
-                    const int r = __shfl_sync(0xffffffffu, row, l0 + i * TI);
-                    const uint64_t at = (uint64_t)max(r, 0) * pitch;
-                    cp_async16_or_zero(ring_k + slot + i * 512, k_src + at, r >= 0);
-                    cp_async16_or_zero((D == 128 && (i & 1) ? ring_v ^ 64u : ring_v) + slot + i * 512, v_src + at, r >= 0);
-                }
+    for (int s = 0; s < S - 1; ++s) {
+        if (s < n_it) {
+            if ((s & 1) == 0) {
+                look_up();
+                park_scales(s >> 1);
             }
-        };
-
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-            if (s < n_it) {
-                if ((s & 1) == 0) {
-                    look_up(s >> 1);
-                    park_scales(s >> 1);
-                }
-                copy(s, s * Kv8Ring<D>::stage_bytes);
-            }
-            cp_async_commit();
+            copy(s, s * Kv8Ring<D, R2>::stage_bytes);
         }
-        uint32_t put_slot = (S - 1) * Kv8Ring<D>::stage_bytes, use_slot = 0;
-        for (int it = 0; it < n_it; ++it) {
-            const int ahead = it + S - 1;
-            const bool looked = ahead < n_it && (ahead & 1) == 0;
-            if (looked) look_up(ahead >> 1);
-            if (ahead < n_it) copy(ahead, put_slot);
-            put_slot = put_slot == (S - 1) * Kv8Ring<D>::stage_bytes ? 0 : put_slot + Kv8Ring<D>::stage_bytes;
-            cp_async_commit();
-            cp_async_wait<S - 1>();
-            __syncwarp();
-            if (tid == 0 && it == 0) TIDAL_STAMP(2);
-            const unsigned char* st = ring + use_slot;
-            use_slot = use_slot == (S - 1) * Kv8Ring<D>::stage_bytes ? 0 : use_slot + Kv8Ring<D>::stage_bytes;
+        cp_async_commit();
+    }
+    uint32_t put_slot = (S - 1) * Kv8Ring<D, R2>::stage_bytes, use_slot = 0;
+
+    List cur;                                                            // of the tile being computed
+    (void)enter(cur, list, first);
+    bool fresh = true;                                                   // a list begins: its queries are to be loaded
+    uint32_t qa[NR][KS][2], ql[QS ? NR : 1][QS ? KS : 1][2];             // Q fragments (lane: head g of each eight), scaled to [2^11, 2^12) per head
+    float qn2[NR][2];                                                    // of heads 2t, 2t+1: undoes the scaling, applies sm_scale, in log2 units
+    float o[NR][KS][4];                                                  // [eight heads][16 elements]: elements 2j, 2j+1 of g*D/8.., heads 2t, 2t+1
+    float m[NR][2], M[NR][2], l[NR][2];
+    for (int it = 0; it < n_it || (p.solo && fresh); ++it) {
+        const int ahead = it + S - 1;
+        const bool looked = ahead < n_it && (ahead & 1) == 0;
+        if (looked) look_up();
+        if (ahead < n_it) copy(ahead, put_slot);
+        put_slot = put_slot == (S - 1) * Kv8Ring<D, R2>::stage_bytes ? 0 : put_slot + Kv8Ring<D, R2>::stage_bytes;
+        cp_async_commit();
+        if (fresh) {
+            fresh = false;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int head = g + 8 * r;
+                const T* qrow = reinterpret_cast<const T*>(p.q) + (row_of(cur.list) + (head < heads ? head : 0)) * D;
+                float f[KS][4], top = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    load4(qrow + (ks >> 2) * 64 + t * 16 + (ks & 3) * 4, f[ks]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float a = fabsf(f[ks][i]);
+                        top = a < INFINITY ? fmaxf(top, a) : top;
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                int sh = 138 - (int)(__float_as_uint(top) >> 23);       // 11 less the exponent of the largest element
+                sh = top == 0.f ? 0 : min(sh, 120);
+                const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+                const float down = p.sm_scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    qn2[r][e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e) * kLog2e;
+                    m[r][e] = M[r][e] = -FLT_MAX;
+                    l[r][e] = 0.f;
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float x0 = f[ks][2 * i] * up, x1 = f[ks][2 * i + 1] * up;
+                        qa[r][ks][i] = head < heads ? pack_f16(x0, x1) : 0u;
+                        if (QS) ql[QS ? r : 0][QS ? ks : 0][i] = head < heads ? pack_f16_rest(x0, x1, qa[r][ks][i]) : 0u;
+                    }
+#pragma unroll
+                for (int j = 0; j < KS; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[r][j][i] = 0.f;
+            }
+            if (n_it == 0) break;                                        // solo: nothing for this warp but an empty share
+        }
+        cp_async_wait<S - 1>();
+        __syncwarp();
+        if (tid == 0 && it == 0) TIDAL_STAMP(2);
+        const unsigned char* st = ring + use_slot;
+        use_slot = use_slot == (S - 1) * Kv8Ring<D, R2>::stage_bytes ? 0 : use_slot + Kv8Ring<D, R2>::stage_bytes;
+        // the pair of tile `it` was looked up this many pairs before the newest one
+        const int age = (min(ahead, n_it - 1) >> 1) - (it >> 1);
+        if (!(it & 1) || (half >> age & 1u)) {
+            const bool all = full >> age & 1u;
             // ---- S^T = K Q^T: tokens g and 8 + g, heads 2t and 2t+1
             float sf[NR][4];
 #pragma unroll
@@ -421,17 +453,15 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
             const float2* scp = &sc_ring[warp][(it >> 1) & (NP - 1)][(it & 1) * kKv8Tile + g];
             const float2 s0 = scp[0], s1 = scp[8];
             const float kf[2] = {s0.x, s1.x}, ev[2] = {s0.y, s1.y};
-            // the pair of tile `it` was looked up ((ahead or the last tile) / 2 - it / 2) pairs before the newest one
-            const bool all = full >> ((min(ahead, n_it - 1) >> 1) - (it >> 1)) & 1u;
             if (p.scores) {
-                const int i0 = w0 + (it >> 1) * TT + (it & 1) * kKv8Tile + g;          // list index of the lane's first token
+                const int i0 = (t0 + (it >> 1) - cur.first) * PAIR + (it & 1) * kKv8Tile + g;      // list index of the lane's first token
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int head = 2 * t + (i & 1) + 8 * r;
                         if (head < heads && kf[i >> 1] >= 0.f)
-                            p.scores[((size_t)b * p.Hq + hq0 + head) * p.score_stride + i0 + (i >> 1) * 8] = sf[r][i] * kf[i >> 1] * qn[r][i & 1];
+                            p.scores[(row_of(cur.list) + head) * p.score_stride + i0 + (i >> 1) * 8] = sf[r][i] * (kf[i >> 1] * qn2[r][i & 1]) * kLn2;
                     }
             }
             // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M for the weights (M is kept less
@@ -537,15 +567,15 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                         if (PS) mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[PS ? r : 0][0], pl[PS ? r : 0][1]);
                     }
             }
-            if (looked) park_scales(ahead >> 1);
-            __syncwarp();                                                // the tile's slot is the next to be filled
         }
-        cp_async_wait<0>();
-        if (tid == 0) TIDAL_STAMP(3);
-
-        // ---- warps of a unit merge through shared memory: o relative to m
-        __syncthreads();
-        float* so = reinterpret_cast<float*>(smem);                      // [warps][rows][D]
+        if (looked) park_scales(ahead >> 1);
+        __syncwarp();                                                    // the tile's slot is the next to be filled
+        // ---- the warp's share of the list ends here
+        const int done = t0 + (it >> 1) + 1;
+        if (!(it & 1) || (done != cur.next && done != t1) || p.solo) continue;
+        const bool whole = done == cur.next && t0 <= cur.first;
+        const int range = cta * TG + tg;
+        const size_t part = ((size_t)unit * (p.ranges + p.lists) + range + cur.list) * p.rows;
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -554,102 +584,151 @@ __global__ void __launch_bounds__(kKv8Warps * 32, (sizeof(T) == 4 && R2) ? 1 : 2
                 float sum = l[r][e];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                if (head >= heads) continue;
+                const float f = fast_exp2(M[r][e] - m[r][e]) * (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f);
+                const size_t out = row_of(cur.list) + head;
                 if (g == 0) {
-                    ml[warp][head][0] = m[r][e];
-                    ml[warp][head][1] = sum;
+                    if (!whole) *reinterpret_cast<float2*>(p.part_ml + (part + head) * 2) = make_float2(m[r][e], sum);
+                    else if (p.lse) p.lse[out] = attn_kv8_lse(m[r][e], sum);
                 }
-                if (head < p.rows) {
-                    const float f = fast_exp2(M[r][e] - m[r][e]);
-                    float* at = so + ((size_t)warp * p.rows + head) * D + g * VB;
 #pragma unroll
-                    for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(o[r][j][e] * f, o[r][j][2 + e] * f);
+                for (int j = 0; j < KS; j += 2) {
+                    const float4 v = make_float4(o[r][j][e] * f, o[r][j][2 + e] * f, o[r][j + 1][e] * f, o[r][j + 1][2 + e] * f);
+                    if (whole) store4(reinterpret_cast<T*>(p.o) + out * D + g * VB + 2 * j, v);
+                    else *reinterpret_cast<float4*>(p.part_o + (part + head) * D + g * VB + 2 * j) = v;
                 }
             }
-        __syncthreads();
-        const int unit_rows = p.HC * p.rows, vecs = unit_rows * (D / 4);
-        const size_t part0 = (size_t)slice * (p.ctas + p.lists);
-        auto put = [&](int ur, int d, float4 acc, float mx, float sum) {
-            const int u = slice * p.HC + ur / p.rows, row = ur % p.rows;
-            const int kh = p.per_head ? 0 : u / p.groups;
-            const int h = p.per_head ? list - b * p.Hq : kh * p.G + (u - kh * p.groups) * p.rows + row;
-            if (!p.per_head && h >= (kh + 1) * p.G) return;
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            store4(reinterpret_cast<T*>(p.o) + ((size_t)b * p.Hq + h) * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-            if (p.lse && d == 0) p.lse[(size_t)b * p.Hq + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
-        };
-        for (int i = tid; i < vecs; i += blockDim.x) {
-            const int ur = i / (D / 4), d = (i - ur * (D / 4)) * 4, uu = ur / p.rows, row = ur - uu * p.rows;
-            float mx = -FLT_MAX, sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < TG; ++k) mx = fmaxf(mx, ml[uu + k * p.HC][row][0]);
-            for (int k = 0; k < TG; ++k) {
-                const int w = uu + k * p.HC;
-                const float f = fast_exp2(ml[w][row][0] - mx);
-                const float4 v = *reinterpret_cast<const float4*>(so + ((size_t)w * p.rows + row) * D + d);
-                sum = fmaf(f, ml[w][row][1], sum);
-                acc.x = fmaf(f, v.x, acc.x);
-                acc.y = fmaf(f, v.y, acc.y);
-                acc.z = fmaf(f, v.z, acc.z);
-                acc.w = fmaf(f, v.w, acc.w);
-            }
-            if (whole) {
-                put(ur, d, acc, mx, sum);
-            } else {
-                const size_t at = (part0 + cta + list) * unit_rows + ur;
-                __stcg(reinterpret_cast<float4*>(p.part_o + at * D + d), acc);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + at * 2), make_float2(mx, sum));
-            }
-        }
-        if (!whole) {
-            // ---- the list is shared by several CTAs: the last of them to arrive merges their parts, in order
-            const int c0 = cta_of(first_tile), parts = cta_of(first_tile + n_tiles - 1) - c0 + 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                uint32_t* cnt = p.arrivals + ((size_t)list * p.slices + slice) * 16;
-                s_last = atomicAdd(cnt, 1u) == (uint32_t)parts - 1u;
-                if (s_last) *cnt = 0u;
-                __threadfence();
-            }
-            __syncthreads();
-            if (s_last) {
-                for (int i = tid; i < vecs; i += blockDim.x) {
-                    const int ur = i / (D / 4), d = (i - ur * (D / 4)) * 4;
-                    const size_t at = (part0 + c0 + list) * unit_rows + ur;
-                    float mx = -FLT_MAX, sum = 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k = 0; k < parts; ++k) mx = fmaxf(mx, __ldcg(p.part_ml + (at + (size_t)k * unit_rows) * 2));
-                    for (int k = 0; k < parts; ++k) {
-                        const float2 s = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (at + (size_t)k * unit_rows) * 2));
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (at + (size_t)k * unit_rows) * D + d));
-                        const float f = fast_exp2(s.x - mx);
-                        sum = fmaf(f, s.y, sum);
-                        acc.x = fmaf(f, v.x, acc.x);
-                        acc.y = fmaf(f, v.y, acc.y);
-                        acc.z = fmaf(f, v.z, acc.z);
-                        acc.w = fmaf(f, v.w, acc.w);
-                    }
-                    put(ur, d, acc, mx, sum);
-                }
-            }
-        }
-        __syncthreads();                                                 // the ring is free for the next segment
-        if (tid == 0) TIDAL_STAMP(4);
-        tile = seg_end;
-        if (p.ragged == 2) break;
+        fresh = true;
+        if (done < t1) (void)enter(cur, cur.list + 1, done);
     }
+    cp_async_wait<0>();
+    if (tid == 0) TIDAL_STAMP(3);
+    if (!p.solo) return;
+
+    // ---- solo: the warps of a unit merge through shared memory, o relative to m
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);                          // [warps][rows][D]
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int head = 2 * t + e + 8 * r;
+            float sum = l[r][e];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (head >= heads) continue;
+            if (g == 0) {
+                ml[warp][head][0] = m[r][e];
+                ml[warp][head][1] = sum;
+            }
+            const float f = fast_exp2(M[r][e] - m[r][e]);
+            float* at = so + ((size_t)warp * p.rows + head) * D + g * VB;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(o[r][j][e] * f, o[r][j][2 + e] * f);
+        }
+    __syncthreads();
+    for (int i = tid; i < heads * (D / 4); i += blockDim.x) {            // one unit to a CTA
+        const int head = i / (D / 4), d = (i - head * (D / 4)) * 4;
+        float mx = -FLT_MAX, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kKv8Warps; ++w) mx = fmaxf(mx, ml[w][head][0]);
+#pragma unroll
+        for (int w = 0; w < kKv8Warps; ++w) {
+            const float f = fast_exp2(ml[w][head][0] - mx);
+            const float4 v = *reinterpret_cast<const float4*>(so + ((size_t)w * p.rows + head) * D + d);
+            sum = fmaf(f, ml[w][head][1], sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const size_t out = row_of(cur.list) + head;
+        store4(reinterpret_cast<T*>(p.o) + out * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (p.lse && d == 0) p.lse[out] = attn_kv8_lse(mx, sum);
+    }
+    if (tid == 0) TIDAL_STAMP(4);
 }
 
+// Adds up the parts of the lists that several warps shared, in the order of their tokens: a group of `split` warps per
+// (list, query head), each warp every split-th part, D/4 lanes to a part.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ AttnKv8Params p, int split) {
+    constexpr int LANES = D / 4, PER = 32 / LANES;       // lanes to a part; parts a warp takes at a time
+    __shared__ float sh_o[8][PER][D];
+    __shared__ float sh_ml[8][PER][2];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, d = lane % LANES * 4;
+    const int per_cta = 8 / split, member = warp % split;
+    const int64_t head_id = (int64_t)blockIdx.x * per_cta + warp / split;        // list-major: (list, query head of the list)
+    const int per_list = p.per_head ? 1 : p.Hq;
+    const bool live = head_id < (int64_t)p.lists * per_list;
+    const int list = live ? (int)(head_id / per_list) : 0, h = live ? (int)(head_id - (int64_t)list * per_list) : 0;
+    const int total = p.ragged ? p.part_prefix[p.lists] : p.pairs_per_list * p.lists;
+    const int begin = p.ragged ? p.part_prefix[list] : list * p.pairs_per_list, end = p.ragged ? p.part_prefix[list + 1] : begin + p.pairs_per_list;
+    const int ranges = min(p.ranges, total);
+    const int r0 = range_of(begin, total, ranges), parts = range_of(end - 1, total, ranges) - r0 + 1;
+    const int kvh = h / p.G, in_kvh = h - kvh * p.G;
+    const int unit = p.per_head ? 0 : kvh * p.groups + in_kvh / p.rows, head = p.per_head ? 0 : in_kvh % p.rows;
+    const size_t part = ((size_t)unit * (p.ranges + p.lists) + r0 + list) * p.rows + head;
+    const size_t step = (size_t)p.rows;
+    const bool work = live && parts > 1;
+    float mx = -FLT_MAX, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (work) {
+        for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, p.part_ml[(part + k * step) * 2]);
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+#pragma unroll 4
+        for (int k = member * PER + sub; k < parts; k += split * PER) {
+            const float2 s = *reinterpret_cast<const float2*>(p.part_ml + (part + k * step) * 2);
+            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (part + k * step) * D + d);
+            const float f = fast_exp2(s.x - mx);
+            sum = fmaf(f, s.y, sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+    }
+    *reinterpret_cast<float4*>(&sh_o[warp][sub][d]) = acc;
+    if (d == 0) sh_ml[warp][sub][0] = sum;
+    __syncthreads();
+    if (!work || member != 0 || sub != 0) return;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    sum = 0.f;
+    for (int w = 0; w < split; ++w)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(&sh_o[warp + w][k][d]);
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            sum += sh_ml[warp + w][k][0];
+        }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t out = p.per_head ? (size_t)list : (size_t)list * p.Hq + h;
+    store4(reinterpret_cast<T*>(p.o) + out * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    if (p.lse && d == 0) p.lse[out] = attn_kv8_lse(mx, sum);
+}
+
+template <typename T, int D, bool R2>
+static int launch_one_kv8(const AttnKv8Params& p, cudaStream_t st) {
+    const size_t smem = Kv8Ring<D, R2>::bytes + (p.ragged && !p.solo ? sizeof(int) * (p.lists + 1) : 0);
+    TIDAL_CUDA_OK(cudaFuncSetAttribute(attn_kv8_kernel<T, D, R2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TIDAL_CUDA_OK(launch_pdl(attn_kv8_kernel<T, D, R2>, dim3((unsigned)p.slices * (unsigned)p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
+    count_launch();
+    return TIDAL_OK;
+}
 template <typename T, int D>
 static int launch_attn_kv8(const AttnKv8Params& p, cudaStream_t st) {
-    const size_t smem = Kv8Ring<D>::bytes + (p.ragged == 1 ? sizeof(int) * (p.lists + 1) : 0);
-    auto go = [&](auto kern) -> int {
-        TIDAL_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        TIDAL_CUDA_OK(launch_pdl(kern, dim3(p.slices, p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
-        count_launch();
-        return TIDAL_OK;
-    };
-    return p.rows > 8 ? go(attn_kv8_kernel<T, D, true>) : go(attn_kv8_kernel<T, D, false>);
+    const int rc = p.rows > 8 ? launch_one_kv8<T, D, true>(p, st) : launch_one_kv8<T, D, false>(p, st);
+    if (rc != TIDAL_OK || p.solo || p.ranges == 1) return rc;
+    const int64_t heads = (int64_t)p.lists * (p.per_head ? 1 : p.Hq);
+    const int split = p.ranges >= 16 * (int64_t)p.lists ? 8 : p.ranges >= 4 * (int64_t)p.lists ? 4 : 1;
+    TIDAL_CUDA_OK(launch_pdl(merge_kv8_kernel<T, D>, dim3((unsigned)((heads + 8 / split - 1) / (8 / split))), dim3(256), 0, st, 1, p, split));
+    count_launch();
+    return TIDAL_OK;
 }
 
 }  // namespace tidal
@@ -692,8 +771,6 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     p.sel_counts = sel ? a->d_sel_counts : nullptr;
     p.scores = a->d_scores; p.score_stride = a->score_stride; p.lse = a->d_lse;
     p.part_o = (float*)((char*)d_ws + L->part_o_off);
-    p.part_ml = (float*)((char*)d_ws + L->part_ml_off);
-    p.arrivals = (uint32_t*)((char*)d_ws + L->xc_off);
     p.status = (uint32_t*)((char*)d_ws + L->status_off);
     p.Hq = a->num_qo_heads; p.Hkv = a->num_kv_heads; p.G = a->num_qo_heads / a->num_kv_heads; p.block = a->block;
     p.sm_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / sqrtf((float)a->head_dim);
@@ -708,25 +785,38 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     const int G = p.per_head ? 1 : p.G;
     p.groups = (G + 15) / 16;
     p.rows = (G + p.groups - 1) / p.groups;
-    const int units = p.per_head ? 1 : p.Hkv * p.groups;
-    // two units to a CTA where there is work for every SM: rows of two heads are adjacent (104 us instead of 111 for 512 MB)
-    p.HC = units % 2 == 0 && lists * units * (int64_t)ntok >= (int64_t)1 << 18 ? 2 : 1;
-    p.slices = units / p.HC;
-    const int TT = 2 * kKv8Tile * (kKv8Warps / p.HC);
-    const bool ragged = sel ? p.sel_counts != nullptr : p.seq_lens != nullptr;
-    p.ragged = !ragged ? 0 : p.lists <= kKv8MaxPrefix ? 1 : 2;
-    p.tiles_per_list = ntok > 0 ? (ntok + TT - 1) / TT : 1;
-    const int64_t most_tiles = (int64_t)p.tiles_per_list * p.lists;
-    TIDAL_REQUIRE(most_tiles <= INT32_MAX, TIDAL_ERR_ARG, "attention_kv8: more than 2^31 tiles of tokens");
-    // two CTAs to an SM share the tiles, at least two tiles each
-    int64_t ctas = 2 * sm_count_cached() / p.slices;
-    ctas = std::max<int64_t>(1, std::min<int64_t>(ctas, (most_tiles + 1) / 2));
-    p.ctas = p.ragged == 2 ? p.lists : (int)ctas;
-    TIDAL_REQUIRE(p.slices <= 65535, TIDAL_ERR_ARG, "attention_kv8: more than 65535 head slices");
-    const size_t parts = (size_t)p.slices * (p.ctas + p.lists) * p.HC * p.rows;
-    TIDAL_REQUIRE(p.ragged == 2 || (L->part_o_off + sizeof(float) * parts * a->head_dim <= L->part_ml_off && L->part_ml_off + sizeof(float) * parts * 2 <= L->hist_off &&
-                                    L->xc_off + sizeof(uint32_t) * 16 * (size_t)p.lists * p.slices <= L->cand_off),
-                  TIDAL_ERR_WORKSPACE, "workspace was sized for a smaller batch/heads/head_dim than this call");
+    p.units = p.per_head ? 1 : p.Hkv * p.groups;
+    p.ragged = sel ? p.sel_counts != nullptr : p.seq_lens != nullptr;
+    p.pairs_per_list = ntok > 0 ? (ntok + 2 * kKv8Tile - 1) / (2 * kKv8Tile) : 1;
+    const int64_t pairs = (int64_t)p.pairs_per_list * p.lists;
+    TIDAL_REQUIRE(pairs <= INT32_MAX, TIDAL_ERR_ARG, "attention_kv8: more than 2^31 pairs of tiles");
+    p.solo = ntok <= kKv8SoloTokens || p.lists > kKv8MaxPrefix;
+    p.HC = 1;
+    while (!p.solo && p.HC < 4 && p.units % (2 * p.HC) == 0) p.HC *= 2;
+    p.slices = p.units / p.HC;
+    const int TG = kKv8Warps / p.HC;
+    if (p.solo) {
+        p.ctas = p.lists;
+    } else {
+        // what is resident (two CTAs to an SM, or one, see attn_kv8_kernel), at least two pairs to a warp, and no more parts than
+        // the workspace holds
+        const int per_sm = p.rows > 8 && (a->dtype == TIDAL_DTYPE_F32 || a->head_dim == 128) ? 1 : 2;
+        int64_t ctas = std::max(1, per_sm * sm_count_cached() / p.slices);
+        ctas = std::min(ctas, (pairs / 2 + TG - 1) / TG);
+        const int64_t room = (int64_t)((L->part_ml_off - L->part_o_off) / (sizeof(float) * a->head_dim)) / ((int64_t)p.units * p.rows) - p.lists;
+        ctas = std::min(ctas, room / TG);
+        TIDAL_REQUIRE(ctas >= 1, TIDAL_ERR_WORKSPACE, "workspace was sized for a smaller batch/heads/head_dim than this call");
+        p.ctas = (int)ctas;
+    }
+    p.ranges = p.ctas * TG;
+    TIDAL_REQUIRE((int64_t)p.ctas * p.slices <= INT32_MAX, TIDAL_ERR_ARG, "attention_kv8: too many lists and heads");
+    // per-row (m, l) of the parts, and in front of them the lists' prefix
+    const size_t prefix_bytes = align_up(sizeof(int32_t) * (size_t)(p.lists + 1), 256);
+    p.part_prefix = (int32_t*)((char*)d_ws + L->part_ml_off);
+    p.part_ml = (float*)((char*)d_ws + L->part_ml_off + prefix_bytes);
+    const size_t parts = (size_t)p.units * (p.ranges + p.lists) * p.rows;
+    TIDAL_REQUIRE(p.solo || L->part_ml_off + prefix_bytes + sizeof(float) * parts * 2 <= L->hist_off, TIDAL_ERR_WORKSPACE,
+                  "workspace was sized for a smaller batch/heads/head_dim than this call");
     cudaStream_t st = (cudaStream_t)stream;
     const bool wide = a->head_dim == 128;
     switch (a->dtype) {
