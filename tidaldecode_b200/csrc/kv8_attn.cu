@@ -38,6 +38,7 @@ namespace tidal {
 
 constexpr int kKv8Warps = 8;
 constexpr int kKv8Tile = 16;             // tokens a warp takes at a time; it looks them up two tiles at a time
+constexpr int kKv8Pair = 2 * kKv8Tile;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself; beyond, a CTA per list
 constexpr int kKv8SoloTokens = 1024;     // lists up to this long go to a CTA each
@@ -59,7 +60,6 @@ struct AttnKv8Params {
     float* lse;
     float* part_o;               // [units][ranges + lists][rows][D]: what a warp has of a list that it shares with others
     float* part_ml;              // [units][ranges + lists][rows][2]
-    int32_t* part_prefix;        // [lists + 1] pairs of tiles before each list, for the merge (ragged)
     uint32_t* status;
     int32_t Hq, Hkv, G, block;
     int32_t lists, per_head;     // token lists: one per sequence, or one per (sequence, query head)
@@ -113,6 +113,31 @@ __device__ __forceinline__ uint32_t pack_f16_rest(float lo, float hi, uint32_t p
 __device__ __forceinline__ int list_len_kv8(const AttnKv8Params& p, int list) {
     if (p.sel_idx) return p.sel_counts ? max(0, min(p.sel_counts[list], p.sel_count)) : p.sel_count;
     return p.seq_lens ? max(0, min(p.seq_lens[list], p.seq_len)) : p.seq_len;
+}
+
+__device__ __forceinline__ int pairs_of_kv8(int len) { return len > 0 ? (len - 1) / kKv8Pair + 1 : 1; }     // an empty list has one empty pair
+// prefix[i] = pairs of the lists before list i, for i <= lists, by the whole CTA (256 threads).
+__device__ __forceinline__ void add_up_lists(const AttnKv8Params& p, int* prefix, int* scan) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (p.lists + blockDim.x - 1) / blockDim.x, first = tid * per, last = min(first + per, p.lists);
+    int sum = 0;
+    for (int i = first; i < last; ++i) sum += pairs_of_kv8(list_len_kv8(p, i));
+    int incl = sum;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int at = incl - sum;
+    for (int i = 0; i < warp; ++i) at += scan[i];
+    for (int i = first; i < last; ++i) {
+        prefix[i] = at;
+        at += pairs_of_kv8(list_len_kv8(p, i));
+        if (i == p.lists - 1) prefix[p.lists] = at;
+    }
+    __syncthreads();
 }
 
 // More than 8 query heads to a unit at D = 128 take all registers of an SM for one CTA; its ring then takes the whole memory.
@@ -184,45 +209,23 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
     const int TG = kKv8Warps / p.HC, uw = warp % p.HC, tg = warp / p.HC;
     const int cta = (int)(blockIdx.x / (uint32_t)p.slices), slice = (int)(blockIdx.x - (uint32_t)cta * (uint32_t)p.slices);
     unsigned char* ring = smem + (size_t)warp * S * Kv8Ring<D, R2>::stage_bytes;
-    constexpr int PAIR = 2 * kKv8Tile;
     if (tid == 0) TIDAL_STAMP(0);
     pdl_wait();
     pdl_launch_dependents();
     if (tid == 0) TIDAL_STAMP(1);
 
     // ---- this warp's range [t0, t1) of pairs
-    auto pairs_of = [&](int len) -> int { return len > 0 ? (len - 1) / PAIR + 1 : 1; };     // an empty list has one empty pair
     int t0, t1, list = 0, first = 0;                                     // `list` starts at pair `first`
     if (p.solo) {
         list = cta;
-        const int n = pairs_of(list_len_kv8(p, list));
+        const int n = pairs_of_kv8(list_len_kv8(p, list));
         t0 = range_begin(tg, n, TG);
         t1 = range_begin(tg + 1, n, TG);
     } else {
         int total;
         if (p.ragged) {
-            const int per = (p.lists + blockDim.x - 1) / blockDim.x, own0 = tid * per;
-            int sum = 0;
-            for (int i = own0; i < min(own0 + per, p.lists); ++i) sum += pairs_of(list_len_kv8(p, i));
-            int incl = sum;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, incl, off);
-                if (lane >= off) incl += y;
-            }
-            if (lane == 31) s_scan[warp] = incl;
-            __syncthreads();
-            int at = incl - sum;
-            for (int i = 0; i < warp; ++i) at += s_scan[i];
-            for (int i = own0; i < min(own0 + per, p.lists); ++i) {
-                prefix[i] = at;
-                at += pairs_of(list_len_kv8(p, i));
-                if (i == p.lists - 1) prefix[p.lists] = at;
-            }
-            __syncthreads();
+            add_up_lists(p, prefix, s_scan);
             total = prefix[p.lists];
-            if (cta == 0 && slice == 0)
-                for (int i = tid; i <= p.lists; i += blockDim.x) p.part_prefix[i] = prefix[i];
         } else {
             total = p.pairs_per_list * p.lists;
         }
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         const int len = list_len_kv8(p, i);
         w.list = i;
         w.first = at;
-        w.next = at + pairs_of(len);
+        w.next = at + pairs_of_kv8(len);
         return len;
     };
     const int unit_kvh = unit / p.groups, unit_hq = unit_kvh * p.G + (unit - unit_kvh * p.groups) * p.rows;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
     List ahead_l;                                                        // of the pair whose entries are loaded next
     int ahead_t = t0, ahead_len = enter(ahead_l, list, first);
     auto fetch_pos = [&]() -> int {
-        const int i = (ahead_t - ahead_l.first) * PAIR + lane;
+        const int i = (ahead_t - ahead_l.first) * kKv8Pair + lane;
         if (ahead_t >= t1 || i >= ahead_len) return INT_MIN;             // no token here
         return p.sel_idx ? max(p.sel_idx[(size_t)ahead_l.list * p.sel_stride + i], -1) : i;
     };
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
             const float2 s0 = scp[0], s1 = scp[8];
             const float kf[2] = {s0.x, s1.x}, ev[2] = {s0.y, s1.y};
             if (p.scores) {
-                const int i0 = (t0 + (it >> 1) - cur.first) * PAIR + (it & 1) * kKv8Tile + g;      // list index of the lane's first token
+                const int i0 = (t0 + (it >> 1) - cur.first) * kKv8Pair + (it & 1) * kKv8Tile + g;      // list index of the lane's first token
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -651,65 +654,105 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
     if (tid == 0) TIDAL_STAMP(4);
 }
 
-// Adds up the parts of the lists that several warps shared, in the order of their tokens: a group of `split` warps per
-// (list, query head), each warp every split-th part, D/4 lanes to a part.
+// Adds up the parts of the lists that several warps shared, in the order of their tokens.  A CTA takes `8 / split` query
+// heads, `split` warps to a head; where there are few heads only blockIdx.y's 32 elements of them, four parts to a warp at a
+// time (one list of 256 K tokens: 10 us less).  What depends on lengths and
+// launch alone is worked out before the attention kernel has ended; then a part costs one trip to L2: each group of lanes
+// keeps a maximum of its own.  (The lengths were there before that kernel began: it waits for its predecessor before it lets
+// this one start.)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ AttnKv8Params p, int split) {
-    constexpr int LANES = D / 4, PER = 32 / LANES;       // lanes to a part; parts a warp takes at a time
-    __shared__ float sh_o[8][PER][D];
-    __shared__ float sh_ml[8][PER][2];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, d = lane % LANES * 4;
+    extern __shared__ int prefix_m[];                    // [lists + 1], ragged
+    __shared__ float sh_o[8][D];
+    __shared__ float sh_ml[8][2];
+    __shared__ int s_scan[8];
+    if (threadIdx.x == 0) TIDAL_STAMP(8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, d = (lane & 7) * 4;
     const int per_cta = 8 / split, member = warp % split;
     const int64_t head_id = (int64_t)blockIdx.x * per_cta + warp / split;        // list-major: (list, query head of the list)
     const int per_list = p.per_head ? 1 : p.Hq;
     const bool live = head_id < (int64_t)p.lists * per_list;
     const int list = live ? (int)(head_id / per_list) : 0, h = live ? (int)(head_id - (int64_t)list * per_list) : 0;
-    const int total = p.ragged ? p.part_prefix[p.lists] : p.pairs_per_list * p.lists;
-    const int begin = p.ragged ? p.part_prefix[list] : list * p.pairs_per_list, end = p.ragged ? p.part_prefix[list + 1] : begin + p.pairs_per_list;
+    if (p.ragged) add_up_lists(p, prefix_m, s_scan);
+    const int total = p.ragged ? prefix_m[p.lists] : p.pairs_per_list * p.lists;
+    const int begin = p.ragged ? prefix_m[list] : list * p.pairs_per_list, end = p.ragged ? prefix_m[list + 1] : begin + p.pairs_per_list;
     const int ranges = min(p.ranges, total);
     const int r0 = range_of(begin, total, ranges), parts = range_of(end - 1, total, ranges) - r0 + 1;
     const int kvh = h / p.G, in_kvh = h - kvh * p.G;
     const int unit = p.per_head ? 0 : kvh * p.groups + in_kvh / p.rows, head = p.per_head ? 0 : in_kvh % p.rows;
     const size_t part = ((size_t)unit * (p.ranges + p.lists) + r0 + list) * p.rows + head;
-    const size_t step = (size_t)p.rows;
+    const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml) + part;
+    const size_t out = p.per_head ? (size_t)list : (size_t)list * p.Hq + h;
     const bool work = live && parts > 1;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) TIDAL_STAMP(9);
+    // the four groups of eight lanes take four parts of one 32-element chunk, or (gridDim.y == 1) the chunks of a head
+    const int chunks = gridDim.y == 1 ? D / 32 : 1, groups = 4 / chunks;
+    const int chunk = sub % chunks, place = sub / chunks;
+    const int at = (blockIdx.y + chunk) * 32 + d;
+    const float* part_o = p.part_o + part * D + at;
     float mx = -FLT_MAX, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (work) {
-        for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, p.part_ml[(part + k * step) * 2]);
+    auto rescale = [&](float to) {
+        const float f = fast_exp2(mx - to);
+        mx = to;
+        sum *= f;
+        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+    };
+    auto add = [&](float m, float l, float4 v) {
+        const float f = fast_exp2(m - mx);
+        sum = fmaf(f, l, sum);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+    };
+    constexpr int K = 4;                                 // parts of a group in flight
+    const int stride = split * groups;
+    for (int k0 = member * groups + place; work && k0 < parts; k0 += stride * K) {
+        float2 s[K];
+        float4 v[K];
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-#pragma unroll 4
-        for (int k = member * PER + sub; k < parts; k += split * PER) {
-            const float2 s = *reinterpret_cast<const float2*>(p.part_ml + (part + k * step) * 2);
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (part + k * step) * D + d);
-            const float f = fast_exp2(s.x - mx);
-            sum = fmaf(f, s.y, sum);
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
+        for (int i = 0; i < K; ++i) {
+            const int k = k0 + i * stride;
+            s[i] = make_float2(-FLT_MAX, 0.f);
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < parts) {
+                s[i] = part_ml[(size_t)k * p.rows];
+                v[i] = *reinterpret_cast<const float4*>(part_o + (size_t)k * p.rows * D);
+            }
+        }
+        rescale(fmaxf(fmaxf(mx, fmaxf(s[0].x, s[1].x)), fmaxf(s[2].x, s[3].x)));
+#pragma unroll
+        for (int i = 0; i < K; ++i) add(s[i].x, s[i].y, v[i]);
+    }
+    float top = mx;
+    for (int off = 8 * chunks; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    rescale(top);
+    for (int off = 8 * chunks; off < 32; off <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+    }
+    if (split > 1) {
+        if (place == 0) *reinterpret_cast<float4*>(&sh_o[warp][chunk * 32 + d]) = acc;
+        if (lane == 0) sh_ml[warp][0] = mx, sh_ml[warp][1] = sum;
+        __syncthreads();
+        if (member == 0 && place == 0) {
+            for (int w = 1; w < split; ++w) top = fmaxf(top, sh_ml[warp + w][0]);
+            rescale(top);
+            for (int w = 1; w < split; ++w) add(sh_ml[warp + w][0], sh_ml[warp + w][1], *reinterpret_cast<const float4*>(&sh_o[warp + w][chunk * 32 + d]));
         }
     }
-    *reinterpret_cast<float4*>(&sh_o[warp][sub][d]) = acc;
-    if (d == 0) sh_ml[warp][sub][0] = sum;
-    __syncthreads();
-    if (!work || member != 0 || sub != 0) return;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    sum = 0.f;
-    for (int w = 0; w < split; ++w)
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const float4 v = *reinterpret_cast<const float4*>(&sh_o[warp + w][k][d]);
-            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-            sum += sh_ml[warp + w][k][0];
-        }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const size_t out = p.per_head ? (size_t)list : (size_t)list * p.Hq + h;
-    store4(reinterpret_cast<T*>(p.o) + out * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-    if (p.lse && d == 0) p.lse[out] = attn_kv8_lse(mx, sum);
+    if (work && member == 0 && place == 0) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store4(reinterpret_cast<T*>(p.o) + out * D + at, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (p.lse && lane == 0 && blockIdx.y == 0) p.lse[out] = attn_kv8_lse(mx, sum);
+    }
+    if (threadIdx.x == 0) TIDAL_STAMP(10);
 }
 
 template <typename T, int D, bool R2>
@@ -726,7 +769,9 @@ static int launch_attn_kv8(const AttnKv8Params& p, cudaStream_t st) {
     if (rc != TIDAL_OK || p.solo || p.ranges == 1) return rc;
     const int64_t heads = (int64_t)p.lists * (p.per_head ? 1 : p.Hq);
     const int split = p.ranges >= 16 * (int64_t)p.lists ? 8 : p.ranges >= 4 * (int64_t)p.lists ? 4 : 1;
-    TIDAL_CUDA_OK(launch_pdl(merge_kv8_kernel<T, D>, dim3((unsigned)((heads + 8 / split - 1) / (8 / split))), dim3(256), 0, st, 1, p, split));
+    const unsigned ctas = (unsigned)((heads + 8 / split - 1) / (8 / split));
+    TIDAL_CUDA_OK(launch_pdl(merge_kv8_kernel<T, D>, dim3(ctas, ctas <= (unsigned)sm_count_cached() ? D / 32 : 1), dim3(256),
+                             p.ragged ? sizeof(int) * (p.lists + 1) : 0, st, 1, p, split));
     count_launch();
     return TIDAL_OK;
 }
@@ -771,6 +816,7 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     p.sel_counts = sel ? a->d_sel_counts : nullptr;
     p.scores = a->d_scores; p.score_stride = a->score_stride; p.lse = a->d_lse;
     p.part_o = (float*)((char*)d_ws + L->part_o_off);
+    p.part_ml = (float*)((char*)d_ws + L->part_ml_off);
     p.status = (uint32_t*)((char*)d_ws + L->status_off);
     p.Hq = a->num_qo_heads; p.Hkv = a->num_kv_heads; p.G = a->num_qo_heads / a->num_kv_heads; p.block = a->block;
     p.sm_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / sqrtf((float)a->head_dim);
@@ -810,12 +856,8 @@ extern "C" int tidal_decode_attention_kv8(const tidal_attn_kv8_args* a, void* d_
     }
     p.ranges = p.ctas * TG;
     TIDAL_REQUIRE((int64_t)p.ctas * p.slices <= INT32_MAX, TIDAL_ERR_ARG, "attention_kv8: too many lists and heads");
-    // per-row (m, l) of the parts, and in front of them the lists' prefix
-    const size_t prefix_bytes = align_up(sizeof(int32_t) * (size_t)(p.lists + 1), 256);
-    p.part_prefix = (int32_t*)((char*)d_ws + L->part_ml_off);
-    p.part_ml = (float*)((char*)d_ws + L->part_ml_off + prefix_bytes);
     const size_t parts = (size_t)p.units * (p.ranges + p.lists) * p.rows;
-    TIDAL_REQUIRE(p.solo || L->part_ml_off + prefix_bytes + sizeof(float) * parts * 2 <= L->hist_off, TIDAL_ERR_WORKSPACE,
+    TIDAL_REQUIRE(p.solo || L->part_ml_off + sizeof(float) * parts * 2 <= L->hist_off, TIDAL_ERR_WORKSPACE,
                   "workspace was sized for a smaller batch/heads/head_dim than this call");
     cudaStream_t st = (cudaStream_t)stream;
     const bool wide = a->head_dim == 128;
