@@ -288,6 +288,51 @@ def test_attention_lists(T, lists, dt, B, Hq, Hkv, D, lens, page, block, k, coun
     _attention_case(T, dt, B, Hq, Hkv, D, lens, page, block, lists=lists, k=k, counts=counts)
 
 
+def test_attention_many_lists(T):
+    """More lists than a CTA adds up, and more sequences than ranges of tokens (warps that cross several lists)."""
+    _attention_case(T, "f16", 130, 16, 4, 64, [50] * 130, 16, 16, lists="per_head", k=40, counts=[i % 41 for i in range(130)])
+    _attention_case(T, "bf16", 300, 2, 1, 64, [1025 + (7 * i) % 300 if i % 5 else i % 3 for i in range(300)], 16, 16)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,lens", [(1, 1, 1, [70001]), (2, 16, 16, [5000, 40001]), (1, 8, 1, [33333]), (3, 32, 2, [1500, 9000, 1]), (1, 24, 2, [20000])])
+def test_attention_long(T, B, Hq, Hkv, lens):
+    """Lists shared by many warps, merged in the order of their parts; units of 1, 8, 12 and 16 heads."""
+    _attention_case(T, "bf16", B, Hq, Hkv, 128, lens, 16, 16)
+    _attention_case(T, "f32", B, Hq, Hkv, 64, lens, 1, 1, want_logits=False)
+
+
+def test_attention_empty_lists(T):
+    """Lists of no entries are not "every token"; a sequence length of zero on the host."""
+    kv, sc = T.alloc_kv8(4, 1, 1, 64)
+    q = torch.randn(2, 3, 64, device="cuda")
+    ws, lse = T.Workspace(2, 3, 64, 1, 1), torch.zeros(2, 3, device="cuda")
+    for kw in (dict(seq_len=2, sel_idx=torch.zeros(2, 0, dtype=torch.int32, device="cuda")), dict(seq_len=2, sel_idx=torch.zeros(2, 3, 0, dtype=torch.int32, device="cuda")),
+               dict(seq_len=0)):
+        o = T.decode_attention_kv8(q, kv, sc, ws=ws, out=torch.full_like(q, 5.0), lse=lse.fill_(1.0), **kw)
+        assert not o.any() and lse.eq(-math.inf).all()
+    assert ws.status() == 0
+
+
+def test_wrapper_refusals(T):
+    kv, sc = T.alloc_kv8(4, 16, 2, 64, 16)
+    q, ws = torch.zeros(1, 4, 64, device="cuda"), T.Workspace(1, 4, 64, 1, 1)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k = torch.zeros(3, 2, 64, device="cuda")
+    for match, call in [
+        ("float8", lambda: T.read_kv8(kv.view(torch.uint8), sc, 4)), ("uint8", lambda: T.read_kv8(kv, sc[:2], 4)), ("divide", lambda: T.read_kv8(kv, torch.zeros(4, 2, 3, 2, dtype=torch.uint8, device="cuda"), 4)),
+        ("range", lambda: T.read_kv8(kv, sc, 4, start=5)), ("out must", lambda: T.read_kv8(kv, sc, 4, out=torch.zeros(4, device="cuda"))), ("page table", lambda: T.read_kv8(kv, sc, 40, page_table=torch.zeros(1, 2, **i32))),
+        ("n_tokens", lambda: T.append_kv8(k, k, kv, sc, batch=2)), ("one dtype", lambda: T.append_kv8(k, k.half(), kv, sc)), ("contiguous", lambda: T.append_kv8(k.transpose(1, 2).contiguous().transpose(1, 2), k, kv, sc)),
+        ("elements", lambda: T.append_kv8(k, k, kv, sc, pos0_dev=torch.zeros(2, **i32))), ("pages", lambda: T.append_kv8(k, k, kv, sc, pos0=62)), ("out of range", lambda: T.append_kv8(k, k, kv, sc, pos0=2 ** 31)),
+        ("not q itself", lambda: T.decode_attention_kv8(q, kv, sc, 4, ws, out=q)), ("sel_idx", lambda: T.decode_attention_kv8(q, kv, sc, 4, ws, sel_counts=torch.zeros(1, **i32))),
+        ("int32", lambda: T.decode_attention_kv8(q, kv, sc, 4, ws, sel_idx=torch.zeros(1, 2, dtype=torch.int64, device="cuda"))), ("scores", lambda: T.decode_attention_kv8(q, kv, sc, 4, ws, scores=torch.zeros(1, 4, device="cuda"))),
+        ("score_stride", lambda: T.decode_attention_kv8(q, kv, sc, 4, ws, scores=torch.zeros(1, 4, 3, device="cuda"))), ("page table", lambda: T.decode_attention_kv8(q, kv, sc, 17, ws, page_table=torch.zeros(1, 1, **i32))),
+        ("contiguous", lambda: T.decode_attention_kv8(q.expand(2, 4, 64), kv, sc, 4, ws)), ("one row per head", lambda: T.accumulate_weights(torch.zeros(1, 4, device="cuda"), q[0, :1], q[0, :1], 4)),
+        ("shapes", lambda: T.evict_pages(torch.zeros(1, 8, device="cuda"), torch.zeros(1, 8, **i32), torch.zeros(1, **i32), 4, out=(torch.zeros(1, 7, device="cuda"), torch.zeros(1, 8, **i32), torch.zeros(1, **i32)))),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("gain,vspread", [(0.0, 0), (1e-4, 0), (40.0, 6), (300.0, 6), (1.0, 100)])
 def test_attention_ranges(T, dt, gain, vspread):

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # TIDAL_B200_LIB names another build of the same library (e.g. one compiled with extra -D flags)
@@ -173,6 +174,25 @@ class EvictArgs(C.Structure):
     ]
 
 
+def packer(cls):
+    """pack(*values): an argument struct as bytes, in native layout from its fields' types.  A third of the time that
+    building the ctypes object takes (0.7 instead of 2.3 us for 20 fields); pointers are numbers, 0 for none."""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    layout = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0q")
+    assert layout.size == C.sizeof(cls), cls
+
+    def pack(*values) -> bytes:
+        try:
+            return layout.pack(*values)
+        except struct.error as e:
+            raise RuntimeError(f"{cls.__name__}: an argument is out of range ({e})") from None
+    return pack
+
+
+pack_append_kv8, pack_read_kv8, pack_attn_kv8 = packer(AppendKv8Args), packer(ReadKv8Args), packer(AttnKv8Args)
+pack_weights, pack_evict = packer(WeightsArgs), packer(EvictArgs)
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -227,12 +247,11 @@ def _load() -> C.CDLL:
     lib.tidal_peer_exchange_reset.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
     lib.tidal_prefill.restype = C.c_int
     lib.tidal_prefill.argtypes = [C.POINTER(PrefillArgs), C.c_void_p]
-    for name, args in (("tidal_append_kv8", AppendKv8Args), ("tidal_read_kv8", ReadKv8Args),
-                       ("tidal_accumulate_weights", WeightsArgs), ("tidal_evict_pages", EvictArgs)):
+    for name in ("tidal_append_kv8", "tidal_read_kv8", "tidal_accumulate_weights", "tidal_evict_pages"):
         getattr(lib, name).restype = C.c_int
-        getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
+        getattr(lib, name).argtypes = [C.c_void_p, C.c_void_p]          # the struct as bytes (packer) or by reference
     lib.tidal_decode_attention_kv8.restype = C.c_int
-    lib.tidal_decode_attention_kv8.argtypes = [C.POINTER(AttnKv8Args), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.tidal_decode_attention_kv8.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     return lib
 
 

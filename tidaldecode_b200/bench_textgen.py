@@ -15,6 +15,7 @@ import time
 
 import torch
 
+from . import ops
 from .llama import LlamaConfig, LlamaForCausalLM
 from .runtime import GraphDecoder
 
@@ -56,12 +57,13 @@ def main():
     ap.add_argument("--random_cache", action="store_true",
                     help="skip prefill: decode from KV caches filled with random values (prefill takes one sequence at a time)")
     ap.add_argument("--torch_linear", action="store_true", help="projections, norms and activations as separate torch/cuBLAS ops")
+    ap.add_argument("--kv_bits", type=int, choices=[8, 16], default=16, help="8: the KV cache in 8 bits with a scale per token and head")
     a = ap.parse_args()
     sel = [] if a.full else a.selection_layers
     m, dtype = build(a.model, sel, a.head_reduce, True)
     max_len = a.context_len + a.decode_len + 8
     rt = GraphDecoder(m, max_seq_len=max_len, token_budget=a.token_budget, dtype=dtype, fused_linear=not a.torch_linear,
-                      batch_size=a.batch)
+                      batch_size=a.batch, kv_bits=a.kv_bits)
     g = torch.Generator().manual_seed(0)
     for it in range(a.iteration):
         torch.cuda.synchronize()
@@ -70,7 +72,12 @@ def main():
             rt.start_from_cache(a.context_len, torch.randint(0, m.vocab_size, (a.batch,), generator=g))
             kv = rt.c.kv_cache
             for layer in range(kv.pool.num_layers):              # N(0,1) keys and values, a layer at a time
-                kv.pool.buf[layer].normal_()
+                if a.kv_bits == 8:
+                    heads, dim = kv.pool.buf.shape[-2:]
+                    k, v = torch.randn(2, a.batch * a.context_len, heads, dim, dtype=dtype, device="cuda")
+                    ops.append_kv8(k, v, kv.buf_layer(layer), kv.scales_layer(layer), batch=a.batch, page_table=kv.page_table)
+                else:
+                    kv.pool.buf[layer].normal_()
         else:
             prompt = torch.randint(0, m.vocab_size, (1, a.context_len), generator=g)
             rt.prefill(prompt)
@@ -88,7 +95,7 @@ def main():
         n = a.decode_len - 2
         print(json.dumps({
             "model": a.model, "batch": a.batch, "context_len": a.context_len, "decode_len": a.decode_len,
-            "token_budget": None if a.full else a.token_budget, "selection_layers": sel, "head_reduce": a.head_reduce, "fused_linear": rt.fused_linear,
+            "token_budget": None if a.full else a.token_budget, "selection_layers": sel, "head_reduce": a.head_reduce, "kv_bits": a.kv_bits, "fused_linear": rt.fused_linear,
             "prefill_s": round(t_prefill, 3), "decode_ms_per_token_device": round(e0.elapsed_time(e1) / n, 4),
             "decode_ms_per_token_wall": round(wall * 1e3 / n, 4), "tokens_per_s": round(a.batch * n / wall, 1),
             "status": rt.c.workspace.status() | int(rt.lin_status.item()), "last_tokens": toks[0, -4:].tolist()}))

@@ -28,6 +28,7 @@
 // Both products have the few query heads as N: with heads as M (16 rows, most of them zero) the first took twice the
 // instructions and twice the registers.  A lane's accumulators belong to heads 2t and 2t+1 throughout.
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -758,7 +759,15 @@ __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ 
 template <typename T, int D, bool R2>
 static int launch_one_kv8(const AttnKv8Params& p, cudaStream_t st) {
     const size_t smem = Kv8Ring<D, R2>::bytes + (p.ragged && !p.solo ? sizeof(int) * (p.lists + 1) : 0);
-    TIDAL_CUDA_OK(cudaFuncSetAttribute(attn_kv8_kernel<T, D, R2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the limit is set to the most that a call may need, once per device (the call costs half a microsecond)
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    TIDAL_CUDA_OK(cudaGetDevice(&dev));
+    if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1u)) {
+        TIDAL_CUDA_OK(cudaFuncSetAttribute(attn_kv8_kernel<T, D, R2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)(Kv8Ring<D, R2>::bytes + sizeof(int) * (kKv8MaxPrefix + 1))));
+        if (dev < 64) set.fetch_or((uint64_t)1 << dev);
+    }
     TIDAL_CUDA_OK(launch_pdl(attn_kv8_kernel<T, D, R2>, dim3((unsigned)p.slices * (unsigned)p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
     count_launch();
     return TIDAL_OK;

@@ -145,9 +145,10 @@ class LlamaForCausalLM(nn.Module):
         self._config = config
 
     def tidal_init(self, page_size: int, max_seq_len: int, token_budget: int = 512, dtype: torch.dtype = torch.float16,
-                   device=torch.device("cuda:0"), batch_size: int = 1):
+                   device=torch.device("cuda:0"), batch_size: int = 1, kv_bits: int = 16, track_weights: bool = False):
         """Allocates the KV pools, the workspace and every per-step buffer; must precede forward
-        (tidal/models/llama.py:616-648)."""
+        (tidal/models/llama.py:616-648).  kv_bits=8 holds the cache in 8 bits; track_weights=True keeps the attention
+        weights that `utils.evict_kv` bounds the cache by."""
         assert self.model.iController is None, "Can't init tidal Controller twice."
         cfg = self._config
         self.model.iController = InferenceController(
@@ -155,7 +156,7 @@ class LlamaForCausalLM(nn.Module):
             head_dim=cfg.hidden_size // cfg.num_attention_heads, page_size=page_size, token_budget=token_budget,
             max_seq_len=max_seq_len, dtype=dtype, device=device, num_kv_heads=cfg.num_key_value_heads,
             batch_size=batch_size, head_reduce=cfg.head_reduce, force_last_token=cfg.force_last_token,
-            layer_alias=cfg.layer_alias)
+            layer_alias=cfg.layer_alias, kv_bits=kv_bits, track_weights=track_weights)
 
     def tidal_clear(self):
         """Forget the cached sequence(s), ready for a new conversation (llama.py:650-656)."""

@@ -473,6 +473,10 @@ def _launch(fn, what: str, index: int, *args) -> None:
             check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _need_on(index: int, *ts) -> None:
     """Every given tensor is contiguous and on device `index`."""
     for t in ts:
@@ -516,7 +520,7 @@ def _kv8_pages(page_table: Optional[torch.Tensor], pages_per_seq: Optional[int],
     """(address, row length) of the page table; without one, sequence b starts at page b * the row length."""
     if page_table is not None:
         return page_table.data_ptr(), _need_rows("page_table", page_table, batch)
-    return None, pages_per_seq if pages_per_seq is not None else pages // max(batch, 1)
+    return 0, pages_per_seq if pages_per_seq is not None else pages // max(batch, 1)
 
 
 def alloc_kv8(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, block: int = 1, device="cuda") -> tuple:
@@ -554,14 +558,16 @@ def append_kv8(
             raise RuntimeError(f"k and v must be [n_tokens, {heads}, {dim}] of one dtype")
         if not t.is_contiguous() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim)):
             raise RuntimeError("the heads of a token must be contiguous in k and v")
+    k_stride = heads * dim if k.is_contiguous() else k.stride(0)
+    v_stride = heads * dim if v.is_contiguous() else v.stride(0)
     if batch < 1 or n % batch:
         raise RuntimeError("n_tokens must be a multiple of batch")
     if n == 0:
         return
     _need_vector("pos0_dev", pos0_dev, batch)
     table, row = _kv8_pages(page_table, pages_per_seq, pages, batch)
-    a = _lib.AppendKv8Args(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), kv.data_ptr(), scales.data_ptr(), table, row,
-                           _ptr(pos0_dev), pos0, batch, n // batch, heads, dim, page_size, block, _dtype_code(k), pages, _ptr(status))
+    a = _lib.pack_append_kv8(k.data_ptr(), v.data_ptr(), k_stride, v_stride, kv.data_ptr(), scales.data_ptr(), table, row,
+                           _addr(pos0_dev), pos0, batch, n // batch, heads, dim, page_size, block, _dtype_code(k), pages, _addr(status))
     _launch(lib.tidal_append_kv8, "tidal_append_kv8", dev, a)
 
 
@@ -584,8 +590,8 @@ def read_kv8(kv: torch.Tensor, scales: torch.Tensor, stop: int, *, start: int = 
     if stop == start:
         return out
     table, row = _kv8_pages(page_table, pages_per_seq, pages, batch)
-    a = _lib.ReadKv8Args(kv.data_ptr(), scales.data_ptr(), table, row, _ptr(seq_lens), out.data_ptr(), start, stop, batch, heads, dim,
-                         page_size, block, _dtype_code(out), pages, _ptr(status))
+    a = _lib.pack_read_kv8(kv.data_ptr(), scales.data_ptr(), table, row, _addr(seq_lens), out.data_ptr(), start, stop, batch, heads, dim,
+                         page_size, block, _dtype_code(out), pages, _addr(status))
     _launch(lib.tidal_read_kv8, "tidal_read_kv8", dev, a)
     return out
 
@@ -622,12 +628,13 @@ def decode_attention_kv8(
         raise RuntimeError("out must be a tensor of q's shape and dtype, and not q itself")
     _need_vector("seq_lens", seq_lens, B)
     table, row = _kv8_pages(page_table, pages_per_seq, pages, B)
-    sel_rows = sel_count = score_stride = 0
+    sel_rows = sel_count = sel_addr = score_stride = 0
     if sel_idx is not None:
         lists = sel_idx.shape
         if sel_idx.dtype != torch.int32 or len(lists) not in (2, 3) or lists[0] != B or (len(lists) == 3 and lists[1] != Hq):
             raise RuntimeError("sel_idx must be int32 [B,k] or [B,Hq,k]")
         sel_rows, sel_count = (1 if len(lists) == 2 else Hq), lists[-1]
+        sel_addr = sel_idx.data_ptr() or q.data_ptr()      # lists of no entries have no address, but are lists all the same
         _need_vector("sel_counts", sel_counts, B * sel_rows)
     elif sel_counts is not None:
         raise RuntimeError("sel_counts needs sel_idx")
@@ -638,8 +645,8 @@ def decode_attention_kv8(
         score_stride = wide[2]
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq)):
         raise RuntimeError("lse must be float32 [B,Hq]")
-    a = _lib.AttnKv8Args(q.data_ptr(), out.data_ptr(), kv.data_ptr(), scales.data_ptr(), table, row, _ptr(seq_lens), seq_len,
-                         _ptr(sel_idx), sel_rows, sel_count, sel_count, _ptr(sel_counts), _ptr(scores), score_stride, _ptr(lse),
+    a = _lib.pack_attn_kv8(q.data_ptr(), out.data_ptr(), kv.data_ptr(), scales.data_ptr(), table, row, _addr(seq_lens), seq_len,
+                         sel_addr, sel_rows, sel_count, sel_count, _addr(sel_counts), _addr(scores), score_stride, _addr(lse),
                          B, Hq, heads, dim, page_size, block, _dtype_code(q), pages, sm_scale)
     _launch(lib.tidal_decode_attention_kv8, "tidal_decode_attention_kv8", dev, a, ws.buf.data_ptr(), ws.nbytes)
     return out
@@ -660,7 +667,7 @@ def accumulate_weights(scores: torch.Tensor, lse: torch.Tensor, weights: torch.T
         raise RuntimeError("lse must be float32 [B,heads]")
     columns = _need_rows("weights", weights, B, torch.float32)
     _need_vector("seq_lens", seq_lens, B)
-    a = _lib.WeightsArgs(scores.data_ptr(), n, lse.data_ptr(), weights.data_ptr(), columns, _ptr(seq_lens), seq_len, B, H, decay)
+    a = _lib.pack_weights(scores.data_ptr(), n, lse.data_ptr(), weights.data_ptr(), columns, _addr(seq_lens), seq_len, B, H, decay)
     _launch(lib.tidal_accumulate_weights, "tidal_accumulate_weights", dev, a)
     return weights
 
@@ -686,7 +693,7 @@ def evict_pages(weights: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
         if len(out) != 3 or _need_rows("out[0]", out[0], rows, torch.float32) != columns or _need_rows("out[1]", out[1], rows) != pages:
             raise RuntimeError("out must be (weights, page_table, seq_lens) of the inputs' shapes and types")
         _need_vector("out[2]", out[2], rows)
-    a = _lib.EvictArgs(weights.data_ptr(), out[0].data_ptr(), columns, page_table.data_ptr(), out[1].data_ptr(), pages, seq_lens.data_ptr(),
+    a = _lib.pack_evict(weights.data_ptr(), out[0].data_ptr(), columns, page_table.data_ptr(), out[1].data_ptr(), pages, seq_lens.data_ptr(),
                        out[2].data_ptr(), columns if max_len is None else max_len, rows, page_size, keep_pages, sink_pages, recent_pages)
     _launch(lib.tidal_evict_pages, "tidal_evict_pages", dev, a)
     return out

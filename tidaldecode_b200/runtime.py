@@ -12,6 +12,9 @@ before capture; the kernels take their lengths from the device (`d_seq_lens`, `p
     rt = GraphDecoder(model, max_seq_len=P + steps)      # model.tidal_init() is done for you
     rt.prefill(prompt_ids)                               # eager, through the attention modules
     tokens = rt.decode(steps)                            # [B, steps] greedy tokens, one replay per token
+
+With kv_bits=8 the cache is held in 8 bits; track_weights=True adds up the selection layers' attention per cached
+token, and rt.evict(keep_tokens) between two decode() calls drops the tokens of least weight — the same graph goes on.
 """
 from __future__ import annotations
 
@@ -21,11 +24,12 @@ import torch
 
 from . import ops
 from .attention import FullAttention, SearchAttention, SparseAttention
+from .utils import evict_kv
 
 
 class GraphDecoder:
     def __init__(self, model, max_seq_len: int, token_budget: Optional[int] = None, dtype: Optional[torch.dtype] = None,
-                 device=None, batch_size: int = 1, fused_linear: bool = True):
+                 device=None, batch_size: int = 1, fused_linear: bool = True, kv_bits: int = 16, track_weights: bool = False):
         self.model = model
         p = next(model.parameters())
         self.dtype = dtype or p.dtype
@@ -34,8 +38,12 @@ class GraphDecoder:
         self.max_seq_len = int(max_seq_len)
         if model.model.iController is None:
             model.tidal_init(page_size=1, max_seq_len=self.max_seq_len, token_budget=token_budget or 256, dtype=self.dtype,
-                             device=self.device, batch_size=batch_size)
+                             device=self.device, batch_size=batch_size, kv_bits=kv_bits, track_weights=track_weights)
         self.c = model.model.iController
+        if (self.c.kv_cache.kv_bits, self.c.weights is not None) != (kv_bits, track_weights):
+            raise RuntimeError("the model's controller was initialised with another kv_bits or track_weights")
+        if track_weights and kv_bits != 8:
+            raise RuntimeError("GraphDecoder keeps attention weights over an 8-bit cache only (kv_bits=8)")
         if self.c.max_seq_len < self.max_seq_len:
             raise RuntimeError("the model's controller was initialised for a shorter max_seq_len")
         if self.c.batch_size != batch_size:
@@ -46,6 +54,8 @@ class GraphDecoder:
         i32 = dict(dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(self.B, **i32)          # tokens per sequence INCLUDING the one being decoded
         self.pos = torch.zeros(self.B, **i32)               # its position
+        self.slot = torch.zeros(self.B, **i32)              # its cache slot: the position less the tokens evicted (8-bit cache)
+        self._evicted = self._done = 0                      # tokens dropped and decoded since the prompt
         self.row_lens = torch.zeros(self.rows, **i32)       # seq_lens per score row
         self.sel_counts = torch.zeros(self.rows, **i32)
         self.tok = torch.zeros(self.B, 1, dtype=torch.int64, device=self.device)
@@ -88,6 +98,8 @@ class GraphDecoder:
         c.kv_cache.reserve(self.max_seq_len)                # page table filled once, never touched again
         self.seq_lens.fill_(P + 1)
         self.pos.fill_(P)
+        self.slot.fill_(P)
+        self._evicted = self._done = 0
         self.row_lens.fill_(P + 1)
         self.tok.copy_(first.view(self.B, 1))
         self.step_idx.zero_()
@@ -109,6 +121,8 @@ class GraphDecoder:
         c.kv_cache._seqlen = seq_len
         self.seq_lens.fill_(seq_len + 1)
         self.pos.fill_(seq_len)
+        self.slot.fill_(seq_len)
+        self._evicted = self._done = 0
         self.row_lens.fill_(seq_len + 1)
         self.tok.copy_(first_tokens.view(self.B, 1).to(self.device))
         self.step_idx.zero_()
@@ -132,7 +146,8 @@ class GraphDecoder:
             pool = c.kv_cache.buf_layer(att.layer_idx)
             rope = dict(pos0_dev=self.pos, page_table=table, rope_theta=att.rope_theta, rope_scale=att.rope_scale,
                         rope_mode=att.rope_mode, inv_freq=att._inv_freq_on(self.device))
-            if fused and h.dtype != torch.float32:
+            kv8 = c.kv_cache.kv_bits == 8
+            if fused and h.dtype != torch.float32 and not kv8:
                 # norm, q|k|v projection, RoPE and the KV append in one launch
                 q = torch.empty(B, att.num_heads, att.head_dim, dtype=h.dtype, device=h.device)
                 ops.qkv_rope_append(h, self._wqkv[li], q, pool, num_kv_heads=att.num_key_value_heads, norm_weight=ln1.weight,
@@ -145,9 +160,28 @@ class GraphDecoder:
                 q = qkv[:, :nq].contiguous().view(B, att.num_heads, att.head_dim)
                 kk = qkv[:, nq:nq + nkv].contiguous().view(B, att.num_key_value_heads, att.head_dim)
                 vv = qkv[:, nq + nkv:].contiguous().view(B, att.num_key_value_heads, att.head_dim)
-                ops.rope_append(q, kk, vv, pool, batch=B, **rope)
+                if kv8:
+                    scales = c.kv_cache.scales_layer(att.layer_idx)
+                    rope.pop("page_table")
+                    ops.rope_append(q, kk, None, None, batch=B, **rope)
+                    ops.append_kv8(kk, vv, pool, scales, batch=B, pos0_dev=self.slot, page_table=table)
+                else:
+                    ops.rope_append(q, kk, vv, pool, batch=B, **rope)
             o = torch.empty_like(q)
-            if isinstance(att, SearchAttention):
+            if kv8:
+                args, kw = (q, pool, scales, self.max_seq_len, ws), dict(out=o, page_table=table, seq_lens=self.seq_lens)
+                if isinstance(att, SearchAttention):
+                    ops.decode_attention_kv8(*args, scores=c.qk_product, lse=c.lse, **kw)
+                    if c.weights is not None:
+                        ops.accumulate_weights(c.qk_product, c.lse, c.weights, self.max_seq_len, seq_lens=self.seq_lens)
+                    ops.topk(c.qk_product, k, ws, n=self.max_seq_len, out_idx=c._topk_indices_full.view(self.rows, -1),
+                             out_val=c._topk_values_full.view(self.rows, -1), force_last=c.force_last_token, row_len=self.row_lens,
+                             out_count=self.sel_counts)
+                elif isinstance(att, SparseAttention):
+                    ops.decode_attention_kv8(*args, sel_idx=c._topk_indices_full, sel_counts=self.sel_counts, **kw)
+                else:
+                    ops.decode_attention_kv8(*args, **kw)
+            elif isinstance(att, SearchAttention):
                 ops.decode_attention(q, pool, self.max_seq_len, ws, out=o, page_table=table, seq_lens=self.seq_lens,
                                      scores=c.qk_product, hist=ws.hist, force_last=c.force_last_token)
                 ops.topk(c.qk_product, k, ws, n=self.max_seq_len, out_idx=c._topk_indices_full.view(self.rows, -1),
@@ -178,6 +212,7 @@ class GraphDecoder:
         self.step_idx.add_(1)
         self.seq_lens.add_(1)
         self.pos.add_(1)
+        self.slot.add_(1)
         self.row_lens.add_(1)
         self.logits = logits
 
@@ -187,7 +222,8 @@ class GraphDecoder:
         """`steps` more greedy tokens (the first call continues after the token `prefill` returned);
         returns those `steps` tokens, [B, steps] on the device."""
         asked = steps
-        if self._prefill_len + 1 + steps > self.max_seq_len:
+        held = self._prefill_len - self._evicted               # tokens of the prompt's account still in the cache
+        if held + max(1, self._done) + steps > self.max_seq_len or self._done + steps > self.out_tokens.shape[1]:
             raise RuntimeError("max_seq_len too small for this many steps")
         if not use_graph:
             for _ in range(steps):
@@ -205,6 +241,16 @@ class GraphDecoder:
                 # the capture pass does not execute: nothing to undo
             for _ in range(steps):
                 self.graph.replay()
-        done = int(self.step_idx.item())
-        self.c.kv_cache._seqlen = self._prefill_len + done      # host bookkeeping catches up with the device
+        done = self._done = int(self.step_idx.item())
+        self.c.kv_cache._seqlen = self._prefill_len + done - self._evicted      # host bookkeeping catches up with the device
         return self.out_tokens[:, done - asked:done]
+
+    def evict(self, keep_tokens: int, sink_tokens: int = 4, recent_tokens: int = 64) -> int:
+        """Between two decode() calls: drop the cached tokens that the selection layers have attended to least until
+        keep_tokens are left (`utils.evict_kv`); returns the tokens dropped per sequence.  The captured graph stays valid:
+        the page table, the lengths and the slots it reads change in place."""
+        dropped = evict_kv(self.c, keep_tokens, sink_tokens, recent_tokens)
+        self._evicted += dropped
+        for t in (self.seq_lens, self.slot, self.row_lens):
+            t.sub_(dropped)
+        return dropped

@@ -9,6 +9,7 @@ controller was built with batch_size B (decode only).
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -22,7 +23,7 @@ from .utils import TensorLayout
 __all__ = [
     "TensorLayout", "KvCache", "InferenceController", "BatchDecodeWithPagedKVCacheWrapper", "append_kv",
     "prefill_forward", "decode_estimate", "decode_topk", "decode_sparse_attn", "rms_norm_forward",
-    "apply_rope_in_place", "rope_append_kv",
+    "apply_rope_in_place", "rope_append_kv", "evict_kv",
 ]
 
 
@@ -50,6 +51,10 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, iController: InferenceController
     The slots were reserved by iController.prepare_metadata()."""
     c = iController
     tps = _tokens_per_seq(k, c)
+    if c.kv_cache.kv_bits == 8:
+        ops.append_kv8(k, v, c.kv_cache.buf_layer(layer_idx), c.kv_cache.scales_layer(layer_idx), batch=c.batch_size,
+                       pos0=c.kv_cache.seqlen - tps, page_table=c.kv_cache.page_table)
+        return
     ops.rope_append(None, k, v, c.kv_cache.buf_layer(layer_idx), batch=c.batch_size, pos0=c.kv_cache.seqlen - tps,
                     page_table=c.kv_cache.page_table, rope_mode=0)
     _update_quest_metadata(c, layer_idx, tps)
@@ -59,12 +64,17 @@ def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, iControlle
                    rope_scale: Optional[float] = None, rope_theta: Optional[float] = None, rope_mode: int = 2,
                    inv_freq: Optional[torch.Tensor] = None):
     """apply_rope_in_place + append_kv in one launch (no reference counterpart: the
-    reference launches RoPE and append separately with a device sync around each)."""
+    reference launches RoPE and append separately with a device sync around each); two launches for an 8-bit cache."""
     c = iController
     tps = _tokens_per_seq(k, c)
-    ops.rope_append(q, k, v, c.kv_cache.buf_layer(layer_idx), batch=c.batch_size, pos0=c.kv_cache.seqlen - tps,
-                    page_table=c.kv_cache.page_table, rope_theta=1e4 if rope_theta is None else rope_theta,
-                    rope_scale=1.0 if rope_scale is None else rope_scale, rope_mode=rope_mode, inv_freq=inv_freq)
+    slot, base = c.kv_cache.seqlen - tps, c.kv_cache.pos_base          # evicted tokens leave the positions as they were
+    rope = dict(batch=c.batch_size, rope_theta=1e4 if rope_theta is None else rope_theta,
+                rope_scale=1.0 if rope_scale is None else rope_scale, rope_mode=rope_mode, inv_freq=inv_freq)
+    if c.kv_cache.kv_bits == 8:
+        ops.rope_append(q, k, None, None, pos0=slot + base, **rope)
+        append_kv(k, v, c, layer_idx)
+        return
+    ops.rope_append(q, k, v, c.kv_cache.buf_layer(layer_idx), pos0=slot + base, page_table=c.kv_cache.page_table, kv_pos_base=base, **rope)
     _update_quest_metadata(c, layer_idx, tps)
 
 
@@ -81,6 +91,11 @@ def prefill_forward(q: torch.Tensor, iController: InferenceController, layer_idx
                     rope_theta: Optional[float] = None) -> torch.Tensor:
     """Causal attention of the prompt over the KV just appended (tidal/utils/__init__.py:131-173)."""
     c = iController
+    if c.kv_cache.kv_bits == 8:
+        n = c.kv_cache.seqlen
+        rows = ops.read_kv8(c.kv_cache.buf_layer(layer_idx), c.kv_cache.scales_layer(layer_idx), n, page_table=c.kv_cache.page_table[:1],
+                            dtype=q.dtype)
+        return ops.prefill(q, rows[0], c._in_order, n)
     return _kernels.prefill_with_paged_kv_cache(q, c.kv_cache.buf_layer(layer_idx), c.kv_indices_with_last,
                                                 c.kv_cache.last_page_len, True, c.layout, False,
                                                 1.0 if rope_scale is None else rope_scale,
@@ -110,7 +125,7 @@ def decode_topk(iController: InferenceController):
     n = c.kv_cache.seqlen
     k = c.inference_token_budget
     ops.topk(c.qk_product, k, c.workspace, n=n, out_idx=c._topk_indices_full, out_val=c._topk_values_full,
-             force_last=c.force_last_token, hist=c.workspace.hist)
+             force_last=c.force_last_token, hist=c.workspace.hist if c.kv_cache.kv_bits != 8 else None)
     c._selection_valid = True
 
 
@@ -130,10 +145,16 @@ def decode_sparse_attn(q: torch.Tensor, iController: InferenceController, layer_
     o = torch.empty_like(q)
     pool = c.kv_cache.buf_layer(layer_idx)
     n = c.kv_cache.seqlen
+    if c.kv_cache.kv_bits == 8:
+        return _decode_attn_kv8(q, o, c, layer_idx, topk_indices, output_qk_product)
     if topk_indices is c.kv_indices_without_last or topk_indices is c.kv_indices_with_last:
         if output_qk_product:
             ops.decode_attention(q, pool, n, c.workspace, out=o, page_table=c.kv_cache.page_table, scores=c.qk_product,
-                                 hist=c.workspace.hist, force_last=c.force_last_token)
+                                 hist=c.workspace.hist, force_last=c.force_last_token, partials=c._partials)
+            if c.weights is not None:
+                m, l, _ = c._partials
+                torch.log2(l, out=c.lse).add_(m).mul_(math.log(2.0))
+                ops.accumulate_weights(c.qk_product, c.lse, c.weights, n)
         else:
             ops.decode_attention(q, pool, n, c.workspace, out=o, page_table=c.kv_cache.page_table)
     elif topk_indices is c.topk_dindices_buffer:
@@ -149,3 +170,35 @@ def decode_sparse_attn(q: torch.Tensor, iController: InferenceController, layer_
                                                                          and c.batch_size == 1) else None,
                                   rope_scale, rope_theta)
     return o
+
+
+def _decode_attn_kv8(q, o, c: InferenceController, layer_idx: int, topk_indices: torch.Tensor, output_qk_product: bool) -> torch.Tensor:
+    """decode_sparse_attn over an 8-bit cache: every cached token, or the set decode_topk chose."""
+    args = (q, c.kv_cache.buf_layer(layer_idx), c.kv_cache.scales_layer(layer_idx), c.kv_cache.seqlen, c.workspace)
+    kw = dict(out=o, page_table=c.kv_cache.page_table)
+    if topk_indices is c.kv_indices_without_last or topk_indices is c.kv_indices_with_last:
+        if not output_qk_product:
+            return ops.decode_attention_kv8(*args, **kw)
+        ops.decode_attention_kv8(*args, scores=c.qk_product, lse=c.lse, **kw)
+        if c.weights is not None:
+            ops.accumulate_weights(c.qk_product, c.lse, c.weights, c.kv_cache.seqlen)
+        return o
+    if topk_indices is not c.topk_dindices_buffer:
+        raise RuntimeError("an 8-bit cache is read by token position: lists of pool pages need a cache in the model's dtype")
+    if not c._selection_valid:
+        raise RuntimeError("sparse layer before a selection layer of this step")
+    if output_qk_product:
+        raise RuntimeError("logits are written by selection layers only")
+    return ops.decode_attention_kv8(*args, sel_idx=c._topk_indices_full, sel_counts=c._counts_full, **kw)
+
+
+def evict_kv(iController: InferenceController, keep_tokens: int, sink_tokens: int = 4, recent_tokens: int = 64) -> int:
+    """Bound the cache between two steps: of every sequence the first sink_tokens, the last recent_tokens and those that the
+    selection layers' queries have attended to most stay, keep_tokens in all; returns the tokens dropped per sequence.
+    Needs a controller built with track_weights=True.  Positions go on counting (later queries and keys are rotated as
+    if nothing had been dropped); the set of the last selection is forgotten.  No reference counterpart."""
+    c = iController
+    if c.weights is None:
+        raise RuntimeError("evict_kv needs InferenceController(..., track_weights=True)")
+    c._selection_valid = False
+    return c.kv_cache.evict(c.weights, keep_tokens, sink_tokens, recent_tokens)

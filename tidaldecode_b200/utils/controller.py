@@ -11,9 +11,12 @@ sequences in lockstep (`batch_size`), how selection scores are reduced
 (`head_reduce`: "none" keeps one top-k set per query head as both reference
 paths do; "sum" adds the logits of all query heads and keeps one shared set),
 whether the newest token is always kept (`force_last_token`, the kernel-path
-rule: decode_page.cuh:326-341, controller.py:140-147), and `layer_alias` to
+rule: decode_page.cuh:326-341, controller.py:140-147), `layer_alias` to
 share one KV buffer among that many layers (the reference hard-wires 4:
-kv_cache.py:84,117; here 1 = no sharing).
+kv_cache.py:84,117; here 1 = no sharing), `kv_bits` = 8 to hold the cache in 8
+bits with a scale per token and head, and `track_weights` to add up, at every
+selection layer, how much attention each cached token has received
+(`weights`), which `utils.evict_kv` bounds the cache by.
 """
 from __future__ import annotations
 
@@ -31,16 +34,20 @@ class InferenceController:
     def __init__(self, num_layers, num_heads, head_dim, page_size, token_budget, max_seq_len, dtype, device,
                  num_kv_heads: Optional[int] = None, batch_size: int = 1, head_reduce: str = "none",
                  force_last_token: bool = True, layer_alias: int = 1, quest_metadata: bool = False,
-                 metadata_page_size: int = 16):
+                 metadata_page_size: int = 16, kv_bits: int = 16, track_weights: bool = False):
         assert page_size == 1, "Only support page_size=1"
         if head_reduce not in ("none", "sum"):
             raise ValueError("head_reduce must be 'none' or 'sum'")
+        if head_reduce == "sum" and (kv_bits == 8 or track_weights):
+            raise ValueError("an 8-bit cache and attention weights need logits per head: head_reduce='none'")
+        if kv_bits == 8 and quest_metadata:
+            raise ValueError("Quest metadata are kept for caches in the model's dtype only")
         num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if num_heads % num_kv_heads:
             raise ValueError(f"num_heads {num_heads} is not a multiple of num_kv_heads {num_kv_heads}")
         self.kv_cache = KvCache(num_layers=num_layers, num_heads=num_kv_heads, head_dim=head_dim, max_seq_len=max_seq_len,
                                 page_size=page_size, dtype=dtype, device=device, layer_alias=layer_alias,
-                                batch_size=batch_size)
+                                batch_size=batch_size, kv_bits=kv_bits)
         # The reference always allocates a second pool for Quest's per-page min/max of the keys
         # (controller.py:31-39); no TidalDecode layer reads it, so it exists only on request
         # (quest_metadata=True: append_kv keeps it up to date, decode_estimate reads it).  One entry per KV
@@ -100,6 +107,18 @@ class InferenceController:
         self.topk_dindices_buffer = None
         self._selection_valid = False
 
+        # 8-bit cache: prefill reads it back as a pool of one-token pages in order
+        self._in_order = torch.arange(max_seq_len, dtype=torch.int32, device=device) if kv_bits == 8 else None
+        # attention weights: per cached token, and what a selection layer leaves for them
+        self.weights = self.lse = self._partials = None
+        if track_weights:
+            f32 = dict(dtype=torch.float32, device=device)
+            self.weights = torch.zeros(batch_size, max_seq_len, **f32)
+            self.lse = torch.zeros(batch_size, num_heads, **f32)
+            if kv_bits != 8:
+                self._partials = (torch.empty(batch_size, num_heads, **f32), torch.empty(batch_size, num_heads, **f32),
+                                  torch.empty(batch_size, num_heads, head_dim, **f32))
+
         self.prefill_latency = []
         self.decode_latency = []
 
@@ -146,3 +165,5 @@ class InferenceController:
     def clean_states(self):
         self.kv_cache.release()
         self._selection_valid = False
+        if self.weights is not None:
+            self.weights.zero_()

@@ -10,16 +10,25 @@ step with the host list by copying only the entries that were added.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
+from .. import ops
 from .utils import TensorLayout
 
 
 class KvPool:
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, capacity: int, block_len: int,
-                 dtype: torch.dtype, device: torch.device):
+                 dtype: torch.dtype, device: torch.device, kv_bits: int = 16):
         self._layout = TensorLayout.NHD
-        self._buf = torch.empty((num_layers, capacity, 2, block_len, num_heads, head_dim), dtype=dtype, device=device)
+        shape = (num_layers, capacity, 2, block_len, num_heads, head_dim)
+        self._scales = None
+        if kv_bits == 8:          # e4m3 codes and one power-of-two scale per token, plane and head (see ops.alloc_kv8)
+            self._buf = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+            self._scales = torch.zeros(shape[:-1], dtype=torch.uint8, device=device)
+        else:
+            self._buf = torch.empty(shape, dtype=dtype, device=device)
         self._free = list(range(capacity - 1, -1, -1))    # pop() hands out the lowest id
 
     @property
@@ -62,10 +71,16 @@ class KvPool:
 
 
 class KvCache:
-    """Key-value cache of `batch_size` sequences that grow in lockstep."""
+    """Key-value cache of `batch_size` sequences that grow in lockstep.
+
+    kv_bits=8 holds the pools in 8 bits (`buf_layer` the codes, `scales_layer` their scales).  `evict` drops the tokens of
+    least weight: slots are renumbered, and a token's position is its slot plus `pos_base`, the tokens dropped so far
+    (of which every sequence has the same number)."""
 
     def __init__(self, num_layers, num_heads, head_dim, max_seq_len: int, page_size, dtype: torch.dtype,
-                 device: torch.device, layer_alias: int = 1, batch_size: int = 1):
+                 device: torch.device, layer_alias: int = 1, batch_size: int = 1, kv_bits: int = 16):
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 16 (the model's dtype) or 8")
         if max_seq_len <= 0:
             raise ValueError("max_seq_len must be positive")
         if layer_alias < 1:
@@ -73,7 +88,10 @@ class KvCache:
         self.batch_size = batch_size
         self._pages_per_seq = (max_seq_len + page_size - 1) // page_size
         self._pool = KvPool(num_layers=max(1, num_layers // layer_alias), num_heads=num_heads, head_dim=head_dim,
-                            capacity=self._pages_per_seq * batch_size, block_len=page_size, dtype=dtype, device=device)
+                            capacity=self._pages_per_seq * batch_size, block_len=page_size, dtype=dtype, device=device,
+                            kv_bits=kv_bits)
+        self.kv_bits = kv_bits
+        self.pos_base = 0
         self._indicies = [[] for _ in range(batch_size)]
         self._seqlen = 0
         self.device = device
@@ -108,6 +126,32 @@ class KvCache:
     def buf_layer(self, layer_idx: int):
         return self._pool.buf[layer_idx % self._pool.num_layers]
 
+    def scales_layer(self, layer_idx: int) -> Optional[torch.Tensor]:
+        """Scales of an 8-bit pool, uint8 [pages, 2, page_size, Hkv]; None for a pool in the model's dtype."""
+        return None if self._pool._scales is None else self._pool._scales[layer_idx % self._pool.num_layers]
+
+    def evict(self, weights: torch.Tensor, keep_tokens: int, sink_tokens: int = 0, recent_tokens: int = 1) -> int:
+        """Keep keep_tokens (a multiple of the page size) tokens of every sequence: the first sink_tokens, the last
+        recent_tokens and the heaviest of the rest by weights fp32 [batch, >= seqlen], which move along in place.
+        Returns the tokens dropped per sequence (0 if the budget covers the cache).  The dropped pages are the next that
+        the sequence grows into.  Blocks: the host's page lists follow the table on the device."""
+        page = self._pool.block_len
+        if keep_tokens % page or sink_tokens % page or recent_tokens % page:
+            raise ValueError(f"keep, sink and recent tokens must be multiples of the page size {page}")
+        if self.num_pages * page <= keep_tokens:
+            return 0
+        lens = torch.full((self.batch_size,), self._seqlen, dtype=torch.int32, device=self.device)
+        ops.evict_pages(weights, self.page_table, lens, keep_tokens // page, page_size=page, max_len=self._seqlen,
+                        sink_pages=sink_tokens // page, recent_pages=max(1, recent_tokens // page))
+        dropped = self._seqlen - int(lens[0])
+        table = self.page_table.cpu()
+        self._stage.copy_(table)
+        for b in range(self.batch_size):
+            self._indicies[b] = table[b, :len(self._indicies[b])].tolist()
+        self._seqlen -= dropped
+        self.pos_base += dropped
+        return dropped
+
     def _ensure_pages(self, n_pages: int) -> int:
         """Allocate until every sequence owns n_pages pages; extends the device page table by the new entries."""
         added = 0
@@ -137,6 +181,7 @@ class KvCache:
 
     def release(self):
         self._seqlen = 0
+        self.pos_base = 0
         for b in range(self.batch_size):
             self._pool.free_blocks(self._indicies[b])
             self._indicies[b].clear()
