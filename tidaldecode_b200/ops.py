@@ -479,12 +479,11 @@ def _addr(t: Optional[torch.Tensor]) -> int:
 
 def _need_on(index: int, *ts) -> None:
     """Every given tensor is contiguous and on device `index`."""
+    if index < 0:
+        raise RuntimeError("tidaldecode_b200 runs on CUDA tensors only (there is no CPU path)")
     for t in ts:
-        if t is not None:
-            if t.get_device() != index or index < 0:
-                raise RuntimeError("tensors must be CUDA tensors of one device (there is no CPU path)")
-            if not t.is_contiguous():
-                raise RuntimeError("tensors must be contiguous")
+        if t is not None and not (t.get_device() == index and t.is_contiguous()):
+            raise RuntimeError("tensors must be contiguous" if t.get_device() == index else "tensors must be CUDA tensors of one device")
 
 
 def _need_rows(name: str, t: Optional[torch.Tensor], rows: int, dtype: torch.dtype = torch.int32) -> int:
@@ -523,6 +522,14 @@ def _kv8_pages(page_table: Optional[torch.Tensor], pages_per_seq: Optional[int],
     return 0, pages_per_seq if pages_per_seq is not None else pages // max(batch, 1)
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the tokens of t [n, heads, dim], whose heads lie next to each other."""
+    rows, heads, last = t.stride()
+    if last != 1 or (t.shape[1] > 1 and heads != t.shape[2]):
+        raise RuntimeError("the heads of a token must be contiguous in k and v")
+    return rows
+
+
 def alloc_kv8(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, block: int = 1, device="cuda") -> tuple:
     """An empty 8-bit KV pool: codes float8_e4m3fn [pages,2,page_size,Hkv,D] (K plane 0, V plane 1) and scales uint8
     [pages,2,page_size/block,Hkv], a byte b standing for 2^(b-127), one per `block` consecutive slots of a page and head."""
@@ -550,16 +557,14 @@ def append_kv8(
     dev = kv.get_device()
     _need_on(dev, kv, scales, pos0_dev, page_table, status)
     pages, page_size, heads, dim, block = _kv8_geometry(kv, scales)
-    n = k.shape[0]
-    for t in (k, v):
-        if t.get_device() != dev:
-            raise RuntimeError("k and v must be CUDA tensors of the pool's device")
-        if t.shape != (n, heads, dim) or t.dtype != k.dtype:
-            raise RuntimeError(f"k and v must be [n_tokens, {heads}, {dim}] of one dtype")
-        if not t.is_contiguous() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim)):
-            raise RuntimeError("the heads of a token must be contiguous in k and v")
-    k_stride = heads * dim if k.is_contiguous() else k.stride(0)
-    v_stride = heads * dim if v.is_contiguous() else v.stride(0)
+    shape = k.shape
+    if k.get_device() != dev or v.get_device() != dev:
+        raise RuntimeError("k and v must be CUDA tensors of the pool's device")
+    if v.shape != shape or len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.dtype != k.dtype:
+        raise RuntimeError(f"k and v must be [n_tokens, {heads}, {dim}] of one dtype")
+    n = shape[0]
+    k_stride = heads * dim if k.is_contiguous() else _row_stride(k)
+    v_stride = heads * dim if v.is_contiguous() else _row_stride(v)
     if batch < 1 or n % batch:
         raise RuntimeError("n_tokens must be a multiple of batch")
     if n == 0:
@@ -584,7 +589,7 @@ def read_kv8(kv: torch.Tensor, scales: torch.Tensor, stop: int, *, start: int = 
         raise RuntimeError(f"bad range [{start}, {stop}) or batch {batch}")
     shape = (batch, stop - start, 2, 1, heads, dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=kv.device)
+        out = kv.new_empty(shape, dtype=dtype)
     elif out.shape != shape:
         raise RuntimeError(f"out must be {list(shape)}")
     if stop == start:
