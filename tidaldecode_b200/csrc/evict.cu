@@ -207,24 +207,27 @@ static __device__ __noinline__ void copy_row(uint32_t* dst, const uint32_t* src,
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictBins = 2048;          // 11-bit digits, from the top: 11 + 11 + 10 bits
-constexpr int kEvictKeys = 48 * 1024;     // page keys a CTA keeps in shared memory; beyond that they are formed anew
+constexpr int kEvictFew = 256;            // keys that are ranked by comparing each with each
+constexpr int kEvictKeys = 47 * 1024;     // page keys a CTA keeps in shared memory; beyond that they are formed anew
 
 // A cluster per row, each of its CTAs with a contiguous part of the row's pages.  The keep - sink - recent heaviest of the
 // pages between the protected ones are found by a radix select over their keys: a histogram per CTA and digit, added up
 // through distributed shared memory by every CTA, so that all know the threshold after one cluster barrier per digit.
 // Equal keys at the threshold go to the lower pages.  A warp owns 32-page groups in order; two walks over them (count,
 // then place) with one prefix over the warps and one over the CTAs between them give every page its place.
-// Bound by latency: three histogram passes and four cluster barriers; the bytes are nothing beside them.
+// Bound by latency: one to three histogram passes, three to four cluster barriers; the bytes are nothing beside them.
 __global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t keys[];
     __shared__ uint32_t hist[3][kEvictBins];
-    __shared__ int sums[32], s_pick[2], s_ties, s_more;
+    __shared__ uint32_t few[kEvictFew];
+    __shared__ int sums[32], s_pick[3], s_ties, s_more, s_few;
     __shared__ int warp_ties[32], warp_more[32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
+    if (tid == 0) s_few = 0;
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.x / C;
@@ -267,8 +270,9 @@ __global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictP
     uint32_t threshold = 0;
     int need = places;                                           // how many of the keys with the threshold's leading digits stay
     if (places > 0) {
+        bool found = false;
 #pragma unroll
-        for (int d = 0; d < 3; ++d) {
+        for (int d = 0; d < 3 && !found; ++d) {
             const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
             for (int i = tid; i < n; i += kEvictThreads) {
                 const int pg = base + i;
@@ -291,10 +295,39 @@ __global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictP
                 const bool high = need <= before + c1;
                 s_pick[0] = bin + (high ? 1 : 0);
                 s_pick[1] = need - before - (high ? 0 : c1);
+                s_pick[2] = high ? c1 : c0;                      // keys with these leading digits
             }
             __syncthreads();
             threshold |= (uint32_t)s_pick[0] << shift;
             need = s_pick[1];
+            if (d == 0 && C == 1 && s_pick[2] <= kEvictFew) {
+                // few keys share the first digit, as a rule: they are ranked against each other, in place of two more histograms
+                // (across CTAs the gathering cost more than it saved: 26 us instead of 20 for 8192 pages)
+                for (int i = tid; i < n; i += kEvictThreads) {
+                    const int pg = base + i;
+                    const uint32_t k = key_of(i);
+                    if (pg >= lo && pg < hi && k >> shift == threshold >> shift) few[atomicAdd(&s_few, 1)] = k;
+                }
+                __syncthreads();
+                const int count = s_few;
+                if (tid < count) {
+                    const uint32_t k = few[tid];
+                    int above = 0, same = 0;
+#pragma unroll 4
+                    for (int i = 0; i < count; ++i) {
+                        above += few[i] > k ? 1 : 0;
+                        same += few[i] == k ? 1 : 0;
+                    }
+                    if (above < need && need <= above + same) {  // the same for every key equal to the threshold
+                        s_pick[0] = (int)k;
+                        s_pick[1] = need - above;
+                    }
+                }
+                __syncthreads();
+                threshold = (uint32_t)s_pick[0];
+                need = s_pick[1];
+                found = true;
+            }
         }
     }
 
@@ -435,7 +468,7 @@ extern "C" int tidal_evict_pages(const tidal_evict_args* a, void* stream) {
     if ((steps & (steps - 1)) == 0) p.page_shift = 31 - __builtin_clz((unsigned)steps);
     // CTAs per row: one CTA takes 1.3 us for every 1024 pages and as much for 4096 weights of longer pages; a second, the
     // fourth and the eighth each add 2 us or more of barriers.  Measured, in us, with 1 / 2 / 4 / 8 CTAs: 4096 single-token
-    // pages 10.1 / 10.8 / 11.7 / 14.5, 16 K 22.5 / 16.7 / 14.5 / 16.5, 128 K 177 / 96 / 43 / 31, 8192 pages of 16 tokens
+    // pages 9.6 / 10.8 / 11.7 / 14.5, 16 K 22.5 / 16.7 / 14.5 / 16.5, 128 K 177 / 96 / 43 / 31, 8192 pages of 16 tokens
     // 37 / 25 / 19 / 20.  Clusters beyond one to an SM would wait for each other (32 rows of 32 K: 19 with 4, 55 with 8).
     const int64_t load = max_pages + (a->page_size > 1 ? a->max_len / 4 : 0);
     int C = load < 6144 ? 1 : load < 12288 ? 2 : load < 45056 ? 4 : 8;
