@@ -154,6 +154,10 @@ def test_append_out_of_range_is_skipped(T):
     K8.append(want, want_s, k[3:].view(1, 1, Hkv, D), k[3:].view(1, 1, Hkv, D), [1], table[3:])
     _same_values(kv, sc, want, want_s)
     assert int(status) == 2
+    status.zero_()
+    T.append_kv8(k.cuda()[:1], k.cuda()[:1], kv, sc, pos0_dev=torch.tensor([-5], dtype=torch.int32, device="cuda"), status=status)
+    _same_values(kv, sc, want, want_s)
+    assert int(status) == 2
 
 
 # -------------------------------------------------------------------------- read

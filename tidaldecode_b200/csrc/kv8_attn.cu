@@ -27,6 +27,11 @@
 //                      accumulator of S^T transposed in 8 x 8 blocks (movmatrix)
 // Both products have the few query heads as N: with heads as M (16 rows, most of them zero) the first took twice the
 // instructions and twice the registers.  A lane's accumulators belong to heads 2t and 2t+1 throughout.
+//
+// Bound by HBM on long contexts: 64 sequences of 16 K tokens, 32/8 heads of 128 (2.1 GB) 331 us, 6.5 TB/s; 16 of them 93 us
+// (5.8 TB/s), of which 6 us pass before the first tile is there, 7 between the first and the last warp's end and 3 in the merge.
+// The same tile loop on the tensor cores' 5th-generation instructions has no use here: at most 16 query rows share a K tile
+// (a tile of tcgen05.mma has 64), and removing either product altogether does not change the time.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -659,10 +664,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 
 // Adds up the parts of the lists that several warps shared, in the order of their tokens.  A CTA takes `8 / split` query
 // heads, `split` warps to a head; where there are few heads only blockIdx.y's 32 elements of them, four parts to a warp at a
-// time (one list of 256 K tokens: 10 us less).  What depends on lengths and
-// launch alone is worked out before the attention kernel has ended; then a part costs one trip to L2: each group of lanes
-// keeps a maximum of its own.  (The lengths were there before that kernel began: it waits for its predecessor before it lets
-// this one start.)
+// time (one list of 256 K tokens: 10 us less).  What depends on lengths and launch alone is worked out before the attention
+// kernel has ended; then a part costs one trip to L2: each group of lanes keeps a maximum of its own.  (The lengths were
+// there before that kernel began: it waits for its predecessor before it lets this one start.)  Bound by latency, 1.5 to 3
+// us behind the attention kernel.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ AttnKv8Params p, int split) {
     extern __shared__ int prefix_m[];                    // [lists + 1], ragged
