@@ -159,7 +159,8 @@ class GraphDecoder:
                     qkv = F.linear(ln1(h), self._wqkv[li])
                 q = qkv[:, :nq].contiguous().view(B, att.num_heads, att.head_dim)
                 kk = qkv[:, nq:nq + nkv].contiguous().view(B, att.num_key_value_heads, att.head_dim)
-                vv = qkv[:, nq + nkv:].contiguous().view(B, att.num_key_value_heads, att.head_dim)
+                vv = qkv[:, nq + nkv:].unflatten(1, (att.num_key_value_heads, att.head_dim))     # append_kv8 takes spaced rows
+                vv = vv if kv8 else vv.contiguous()
                 if kv8:
                     scales = c.kv_cache.scales_layer(att.layer_idx)
                     rope.pop("page_table")
