@@ -305,6 +305,27 @@ def test_attention_long(T, B, Hq, Hkv, lens):
     _attention_case(T, "f32", B, Hq, Hkv, 64, lens, 1, 1, want_logits=False)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(1, 1, 64), (8, 1, 128), (12, 1, 128), (24, 1, 64)])
+def test_attention_long_sums_are_rounded_to_nearest(T, Hq, Hkv, D):
+    """fp32, many tokens to a warp (all sequences list the same pages), every weight equal and no value negative: the
+    logits, the weights and a tile's 16 products are exact, so what is left are n / 16 additions.  Rounded to nearest,
+    each is off by a uniform error of up to 2^-24 of a sum that grows evenly, sqrt(n / 16) / 3 * 2^-24 of the result in
+    the root mean square; twice that is allowed, and 2^-22 for the merge and the division.  Sums that are cut off would
+    be off by about n / 32 * 2^-24."""
+    g = _gen(D + Hq)
+    n, page, B = 20000, 16, 400
+    table, pages = _table(g, 1, n // page)
+    codes, scales = _pool(g, pages, page, page, Hkv, D)
+    codes[:, 1] &= 127
+    scales[:, 1] = 120
+    want = K8.values(codes, scales)[table[0].long(), 1].view(n, Hkv, D).double().mean(0).repeat_interleave(Hq // Hkv, 0)
+    ws = T.Workspace(B, Hq, D, 1, 1)
+    o = T.decode_attention_kv8(torch.zeros(B, Hq, D, device="cuda"), codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), n, ws,
+                               page_table=table.cuda().expand(B, -1).contiguous())
+    off = (o.cpu().double() - want).flatten(1).norm(dim=1) / want.norm()
+    assert ws.status() == 0 and off.max() <= 2 * math.sqrt(n / 16) / 3 * 2.0 ** -24 + 2.0 ** -22, off.max()
+
+
 def test_attention_empty_lists(T):
     """Lists of no entries are not "every token"; a sequence length of zero on the host."""
     kv, sc = T.alloc_kv8(4, 1, 1, 64)

@@ -13,7 +13,12 @@
 // bf16 and fp16 rows exactly (elements 2^25 below the largest lose bits); fp32 rows are split into two fp16 terms (22
 // bits).  Weights are scaled to at most 2^14 (tokens down to 2^-38 of the heaviest still count) and rounded to fp16: half a
 // step is 2^-12, next to 2^-9 for a bf16 result; for fp16 and fp32 results a second fp16 term carries the remainder.
-// Accumulators, maxima and sums are fp32.
+// Accumulators, maxima and sums are fp32.  The tensor cores cut a sum's last bits off, and over a long chain that adds up (to
+// 8e-6 of a result after 30 K tokens, 1.7e-5 after 7 K tokens to a warp).  So where the result is fp32 the chain is short, and
+// what it gives is added by ordinary additions: after every tile where registers allow, after kKv8Chain tiles, with
+// the sums in local memory, where they do not (D = 128, up to eight heads to a unit).  8 sequences, one head to a unit, 8192
+// tokens, D = 128: 38.6 us unsplit, 53 after every tile (spills), 39.3 parked; 16 heads to a unit, 16384 tokens, D = 64: 27.6,
+// 28.0, 30.8.  For 16-bit results the rounding of the result is a hundred times larger, and the chain stays whole.
 //
 // Data movement.  Every warp has a ring of tiles of its own in shared memory, filled with cp.async, 16 bytes to a lane and a
 // whole row to adjacent lanes (with the two pieces of a 32-byte sector four lanes apart, sectors were fetched twice: 6.0
@@ -43,6 +48,7 @@
 namespace tidal {
 
 constexpr int kKv8Warps = 8;
+constexpr int kKv8Chain = 16;               // tiles whose values tensor cores add up before their sum is parked
 constexpr int kKv8Tile = 16;             // tokens a warp takes at a time; it looks them up two tiles at a time
 constexpr int kKv8Pair = 2 * kKv8Tile;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -96,6 +102,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The product alone.
+__device__ __forceinline__ void mma_f16_fresh(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 // An 8 x 8 matrix of 16-bit elements, lane (g, t) holding row g, columns 2t and 2t+1, transposed.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -205,6 +217,7 @@ template <typename T, int D, bool R2>    // R2: more than 8 query heads to a uni
 __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 128) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
     constexpr bool QS = sizeof(T) == 4, PS = !std::is_same<T, __nv_bfloat16>::value;
     constexpr int S = Kv8Ring<D, R2>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
+    constexpr bool park = QS && D == 128 && !R2;
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int NP = S <= 4 ? 2 : 4;       // pairs of tiles whose scales are kept: a slot is refilled S - 2 NP <= 0 tiles after its last use
     // per token: scale of K (-1: no token) and exponent of the scale of V (-inf: the block reads as zeros)
@@ -378,6 +391,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
     float qn2[NR][2];                                                    // of heads 2t, 2t+1: undoes the scaling, applies sm_scale, in log2 units
     float o[NR][KS][4];                                                  // [eight heads][16 elements]: elements 2j, 2j+1 of g*D/8.., heads 2t, 2t+1
     float m[NR][2], M[NR][2], l[NR][2];
+    volatile float parked[NR * KS * 4];                                  // sums of earlier tiles of the list
+    bool any_parked = false;
+    auto unpark = [&]() {
+        if (!park || !any_parked) return;
+#pragma unroll
+        for (int i = 0; i < NR * KS * 4; ++i) o[i / (4 * KS)][i / 4 % KS][i % 4] += parked[i];
+    };
     for (int it = 0; it < n_it || (p.solo && fresh); ++it) {
         const int ahead = it + S - 1;
         const bool looked = ahead < n_it && (ahead & 1) == 0;
@@ -386,7 +406,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         put_slot = put_slot == (S - 1) * Kv8Ring<D, R2>::stage_bytes ? 0 : put_slot + Kv8Ring<D, R2>::stage_bytes;
         cp_async_commit();
         if (fresh) {
-            fresh = false;
+            fresh = any_parked = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 const int head = g + 8 * r;
@@ -427,6 +447,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                     for (int i = 0; i < 4; ++i) o[r][j][i] = 0.f;
             }
             if (n_it == 0) break;                                        // solo: nothing for this warp but an empty share
+        } else if (park && it % kKv8Chain == 0) {
+            unpark();
+#pragma unroll
+            for (int i = 0; i < NR * KS * 4; ++i) {
+                parked[i] = o[i / (4 * KS)][i / 4 % KS][i % 4];
+                o[i / (4 * KS)][i / 4 % KS][i % 4] = 0.f;
+            }
+            any_parked = true;
         }
         cp_async_wait<S - 1>();
         __syncwarp();
@@ -438,11 +466,11 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         if (!(it & 1) || (half >> age & 1u)) {
             const bool all = full >> age & 1u;
             // ---- S^T = K Q^T: tokens g and 8 + g, heads 2t and 2t+1
-            float sf[NR][4];
+            float sf[NR][4], sl[QS ? NR : 1][4];                         // the second terms' products have a chain of their own
 #pragma unroll
             for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sf[r][i] = 0.f;
+                for (int i = 0; i < 4; ++i) sf[r][i] = sl[QS ? r : 0][i] = 0.f;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const uint4 k0 = *reinterpret_cast<const uint4*>(st + (k_off ^ c * 64)), k1 = *reinterpret_cast<const uint4*>(st + 8 * D + (k_off ^ c * 64));
@@ -456,9 +484,15 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
                         mma_f16(sf[r], a[0], a[1], a[2], a[3], qa[r][ks][0], qa[r][ks][1]);
-                        if (QS) mma_f16(sf[r], a[0], a[1], a[2], a[3], ql[QS ? r : 0][QS ? ks : 0][0], ql[QS ? r : 0][QS ? ks : 0][1]);
+                        if (QS) mma_f16(sl[QS ? r : 0], a[0], a[1], a[2], a[3], ql[QS ? r : 0][QS ? ks : 0][0], ql[QS ? r : 0][QS ? ks : 0][1]);
                     }
                 }
+            }
+            if (QS) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sf[r][i] += sl[QS ? r : 0][i];
             }
             // ---- scales of the two tokens; value i of a lane: token g + 8 (i / 2), head 2t + i % 2
             const float2* scp = &sc_ring[warp][(it >> 1) & (NP - 1)][(it & 1) * kKv8Tile + g];
@@ -531,6 +565,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                             o[r][j][e] *= a;
                             o[r][j][2 + e] *= a;
                         }
+                        if (park && any_parked) {
+#pragma unroll
+                            for (int j = 0; j < KS; ++j) {
+                                parked[(r * KS + j) * 4 + e] = parked[(r * KS + j) * 4 + e] * a;
+                                parked[(r * KS + j) * 4 + 2 + e] = parked[(r * KS + j) * 4 + 2 + e] * a;
+                            }
+                        }
                     }
                 exponents();
             }
@@ -574,6 +615,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
+                        if (QS && !park) {
+                            float part[4];
+                            mma_f16_fresh(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[PS ? r : 0][0], pl[PS ? r : 0][1]);
+                            mma_f16(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[r][2 * w + e][i] += part[i];
+                            continue;
+                        }
                         mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
                         if (PS) mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[PS ? r : 0][0], pl[PS ? r : 0][1]);
                     }
@@ -584,6 +633,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         // ---- the warp's share of the list ends here
         const int done = t0 + (it >> 1) + 1;
         if (!(it & 1) || (done != cur.next && done != t1) || p.solo) continue;
+        unpark();
         const bool whole = done == cur.next && t0 <= cur.first;
         const int range = cta * TG + tg;
         const size_t part = ((size_t)unit * (p.ranges + p.lists) + range + cur.list) * p.rows;
@@ -617,6 +667,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
     if (!p.solo) return;
 
     // ---- solo: the warps of a unit merge through shared memory, o relative to m
+    unpark();
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem);                          // [warps][rows][D]
 #pragma unroll
