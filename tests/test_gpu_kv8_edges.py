@@ -1,0 +1,67 @@
+"""Edges of the 8-bit KV cache operators: results to the last bit of their type, the ends of the ranges of scales, weights and
+starts, and calls that come after an eviction.  Against the definitions in 64 bits (oracle/kv8_oracle.py)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv8_oracle as K8
+
+pytestmark = pytest.mark.gpu
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+LOG2E = 1.4426950408889634
+
+
+@pytest.fixture(scope="module")
+def T():
+    import tidaldecode_b200.ops as ops
+    return ops
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _half_step(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Half the distance between the type's numbers in x's binade (of the subnormal numbers below the smallest normal one)."""
+    info = torch.finfo(dtype)
+    e = torch.frexp(x.abs().clamp(min=info.smallest_normal))[1].double() - 1
+    return 2.0 ** e * info.eps / 2
+
+
+# --------------------------------------------------------------- attention: last bits
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 12, 1), (128, 16, 1)])
+def test_attention_rounds_16_bit_results_once(T, dt, D, Hq, Hkv):
+    """A 16-bit result is the 64-bit one rounded to its type: off by half a step and by what 32-bit arithmetic loses.  The
+    softmax weights have no rounding of their own beyond that: held in two fp16 terms they are off by 2^-22.  With
+    dot = max_j sum_d |q_d k_jd| sm and A = sum_j p_j |v_j|, for up to 33 tokens:
+        dx = 20 * 2^-23 * dot           logits (8 to 16 fp32 additions of exact products, the scale factors)
+        de = dx + 2^-22 (2 + max|x| log2 e)     the exponential and its argument
+        t  = A (2 de + 2^-22 + 40 * 2^-23) + 2^-38 U     weights and denominator, their two terms, sums, fp16's last step
+    and the result lies within t + half a step, of the binade that holds |o| + t.  (One fp16 term: 2^-12 in place of 2^-22,
+    ten times t here.)"""
+    g = _gen(D + Hq)
+    lens = list(range(1, 34))
+    B, page, sm, G = len(lens), 16, 1 / math.sqrt(D), Hq // Hkv
+    codes = torch.randint(0, 256, (3 * B, 2, page, Hkv, D), generator=g).to(torch.uint8)
+    codes[codes & 127 == 127] = 0
+    scales = torch.full((3 * B, 2, 1, Hkv), 121, dtype=torch.uint8)
+    table = torch.randperm(3 * B, generator=g).view(B, 3).to(torch.int32)
+    q = (0.1 * torch.randn(B, Hq, D, generator=g)).to(DT[dt])
+    ws = T.Workspace(B, Hq, D, 1, 1)
+    o = T.decode_attention_kv8(q.cuda(), codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), max(lens), ws, page_table=table.cuda(),
+                               seq_lens=torch.tensor(lens, dtype=torch.int32, device="cuda")).cpu().double()
+    assert ws.status() == 0
+    vals = K8.values(codes, scales)
+    for b, n in enumerate(lens):
+        pos = torch.arange(n)
+        kv = vals[table[b].long()[pos // page], :, pos % page]
+        for h in range(Hq):
+            want, x, _, A, dot, U = K8.attention(q[b, h], kv[:, 0, h // G], kv[:, 1, h // G], sm, torch.full((n,), 2.0 ** -6, dtype=torch.float64))
+            de = 20 * 2.0 ** -23 * dot + 2.0 ** -22 * (2 + float(x.abs().max()) * LOG2E)
+            t = A * (2 * de + 2.0 ** -22 + 40 * 2.0 ** -23) + 2.0 ** -38 * U
+            tol = t + _half_step(want.abs() + t, DT[dt])
+            assert ((o[b, h] - want).abs() <= tol).all(), (n, h, float(((o[b, h] - want).abs() / tol).max()))
