@@ -65,3 +65,25 @@ def test_attention_rounds_16_bit_results_once(T, dt, D, Hq, Hkv):
             t = A * (2 * de + 2.0 ** -22 + 40 * 2.0 ** -23) + 2.0 ** -38 * U
             tol = t + _half_step(want.abs() + t, DT[dt])
             assert ((o[b, h] - want).abs() <= tol).all(), (n, h, float(((o[b, h] - want).abs() / tol).max()))
+
+
+# ------------------------------------------------------------------ append: any start
+@pytest.mark.parametrize("page,block", [(1, 1), (4, 4), (6, 3)])
+def test_append_starts_at_the_end_of_the_integers(T, page, block):
+    """Starts on the device whose tokens run past 2^31 - 1: nothing is read or written for them, they are reported, and
+    the other sequence is stored."""
+    g = _gen(20)
+    Hkv, D, n = 2, 64, 4
+    top = 2 ** 31 - 1
+    pos = torch.tensor([top, top - 1, 3, top - 2, top - 5], dtype=torch.int32)
+    B, per_seq = len(pos), 12 // page
+    codes = torch.randint(0, 127, (B * per_seq, 2, page, Hkv, D), generator=g).to(torch.uint8)
+    scales = torch.full((B * per_seq, 2, page // block, Hkv), 121, dtype=torch.uint8)
+    k = torch.randn(B * n, Hkv, D, generator=g)
+    kv, sc, status = codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    T.append_kv8(k.cuda(), k.cuda(), kv, sc, batch=B, pos0_dev=pos.cuda(), status=status)
+    want, want_s = K8.values(codes, scales), scales.long()
+    mine = k.view(B, n, Hkv, D)[2:3]
+    K8.append(want, want_s, mine, mine, [3], torch.arange(B * per_seq).view(B, per_seq)[2:3])
+    assert torch.equal(sc.cpu().long(), want_s) and torch.equal(K8.values(kv.cpu(), sc.cpu()), want)
+    assert int(status) == 2

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) append_kv8_kernel(const AppendKv8Params p
     const int b = (int)((rest >> 1) / (uint32_t)p.blocks_per_seq), j = (int)((rest >> 1) - (uint32_t)b * (uint32_t)p.blocks_per_seq);
     const int pos0 = p.pos0_dev ? p.pos0_dev[b] : p.pos0;
     const int64_t end = (int64_t)pos0 + p.T;
-    const int64_t s0 = pos0 < 0 ? -1 : (int64_t)(pos0 / p.block + j) * p.block;      // first slot of the block
+    const int64_t s0 = pos0 < 0 ? -1 : ((int64_t)(pos0 / p.block) + j) * p.block;    // first slot of the block (a start may be any number)
     const bool in = live && pos0 >= 0 && s0 < end && s0 <= INT32_MAX - p.block;
     const int lo = in && pos0 > s0 ? (int)(pos0 - s0) : 0;                            // rows [0, lo) hold codes already,
     const int hi = in ? (int)min((int64_t)p.block, end - s0) : 0;                     // rows [lo, hi) are new
