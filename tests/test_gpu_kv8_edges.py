@@ -87,3 +87,29 @@ def test_append_starts_at_the_end_of_the_integers(T, page, block):
     K8.append(want, want_s, mine, mine, [3], torch.arange(B * per_seq).view(B, per_seq)[2:3])
     assert torch.equal(sc.cpu().long(), want_s) and torch.equal(K8.values(kv.cpu(), sc.cpu()), want)
     assert int(status) == 2
+
+
+@pytest.mark.parametrize("e", [-110, -16, -15, 15, 23, 24, 25, 26, 60, 119])
+def test_append_f16_rows_behind_tokens_of_any_scale(T, e):
+    """A block whose first token came in 32 bits and has scale 2^e, then 16-bit rows, among them the largest, infinite and
+    NaN ones: codes and scales bit for bit.  From 2^25 on only magnitudes above 2^(e - 10) are more than zero."""
+    g = _gen(21)
+    D = 64
+    first = torch.randn(1, 1, 1, D, generator=g)
+    first[0, 0, 0, 0] = 448.0
+    first = (first.clamp(-448, 448).double() * 2.0 ** e).float()
+    rows = (torch.randn(1, 3, 1, D, generator=g) * 2.0 ** 10).half()
+    rows[0, 0, 0, :8] = torch.tensor([65504.0, -65504.0, 40000.0, 32768.0, 32800.0, 2.0 ** -24, -0.0, 60000.0])
+    rows[0, 1, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 50000.0])
+    rows[0, 2] *= 2.0 ** -20
+    codes, scales = torch.zeros(1, 2, 4, 1, D, dtype=torch.uint8), torch.zeros(1, 2, 1, 1, dtype=torch.uint8)
+    want, want_s = K8.values(codes, scales), scales.long()
+    kv, sc = codes.cuda().view(torch.float8_e4m3fn), scales.cuda()
+    K8.append(want, want_s, first, first, [0], [[0]])
+    assert want_s.eq(e + 127).all()
+    T.append_kv8(first[0].cuda(), first[0].cuda(), kv, sc)
+    K8.append(want, want_s, rows, rows, [1], [[0]])
+    T.append_kv8(rows[0].cuda(), rows[0].cuda(), kv, sc, pos0=1)
+    got = K8.values(kv.cpu(), sc.cpu())
+    assert torch.equal(sc.cpu().long(), want_s) and torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))

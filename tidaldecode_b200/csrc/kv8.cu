@@ -76,11 +76,12 @@ __device__ __forceinline__ uint2 codes8(const float* x, float inv) {
     return make_uint2(pack_e4m3(x[0] * inv, x[1] * inv) | pack_e4m3(x[2] * inv, x[3] * inv) << 16,
                       pack_e4m3(x[4] * inv, x[5] * inv) | pack_e4m3(x[6] * inv, x[7] * inv) << 16);
 }
-// Codes of eight stored elements times inv, a power of two.  fp16 rows stay in pairs while inv is an fp16 number: the product
-// is exact, or below 2^-14 and then a zero code either way.
+// Codes of eight stored elements times inv, a power of two.  fp16 rows stay in pairs while inv is an fp16 number (2^-24 ..
+// 2^15; the scale of a block that holds tokens of another type may ask for less): the product is exact, or below 2^-14 and
+// then a zero code either way.
 template <typename T>
 __device__ __forceinline__ uint2 codes8(const Raw8<T>& r, float inv) {
-    if (std::is_same<T, __half>::value && inv <= 32768.f) {
+    if (std::is_same<T, __half>::value && inv >= 0x1p-24f && inv <= 0x1p15f) {
         const __half2 k = __float2half2_rn(inv);
         uint32_t c[4];
 #pragma unroll
