@@ -113,3 +113,16 @@ def test_append_f16_rows_behind_tokens_of_any_scale(T, e):
     got = K8.values(kv.cpu(), sc.cpu())
     assert torch.equal(sc.cpu().long(), want_s) and torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+# -------------------------------------------------------------------------- read-back
+def test_read_leaves_rows_of_negative_lengths(T):
+    """A length below zero, down to the smallest integer, holds no rows: they are left as they were."""
+    g = _gen(22)
+    codes, scales = torch.randint(0, 127, (40, 2, 1, 1, 64), generator=g).to(torch.uint8), torch.full((40, 2, 1, 1), 121, dtype=torch.uint8)
+    lens = torch.tensor([-2 ** 31, -2 ** 31 + 6, -1, 9], dtype=torch.int32)
+    out = torch.full((4, 3, 2, 1, 1, 64), -7.0, device="cuda")
+    T.read_kv8(codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), 10, start=7, batch=4, seq_lens=lens.cuda(), out=out)
+    want = torch.full((4, 3, 2, 64), -7.0, dtype=torch.float64)
+    want[3, :2] = K8.values(codes, scales)[37:39, :, 0, 0]
+    assert torch.equal(out.cpu().double()[:, :, :, 0, 0], want)

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) read_kv8_kernel(const ReadKv8Params p) {
     const int v = blockIdx.z * 256 + (p.toks > 1 ? (int)threadIdx.x - sub * p.per_tok : (int)threadIdx.x);
     if (v >= p.per_tok || (p.toks > 1 && sub >= p.toks)) return;
     const int hp = v / VPR, plane = hp >= p.Hkv ? 1 : 0, h = hp - plane * p.Hkv;
-    const int last = p.seq_lens ? min(p.n, p.seq_lens[b] - p.start) : p.n;
+    const int last = p.seq_lens ? (int)min((int64_t)p.n, max((int64_t)p.seq_lens[b] - p.start, (int64_t)0)) : p.n;
     const int tok0 = (int)blockIdx.x * kReadSteps * p.toks + (p.toks > 1 ? sub : 0);
     const int32_t* table = p.map.page_table ? p.map.page_table + (size_t)b * p.map.pt_stride : nullptr;
     const int64_t page0 = (int64_t)b * p.map.pt_stride;
