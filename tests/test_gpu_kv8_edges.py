@@ -126,3 +126,69 @@ def test_read_leaves_rows_of_negative_lengths(T):
     want = torch.full((4, 3, 2, 64), -7.0, dtype=torch.float64)
     want[3, :2] = K8.values(codes, scales)[37:39, :, 0, 0]
     assert torch.equal(out.cpu().double()[:, :, :, 0, 0], want)
+
+
+# ------------------------------------------------------------ attention: smallest results
+def _attend_one(T, dt, q, codes, scales, n, sm):
+    """One KV head, one-token pages in order: the output [Hq, D] in 64 bits and (want, A, U, x, dot) per query head."""
+    Hq, D = q.shape
+    ws = T.Workspace(1, Hq, D, 1, 1)
+    o = T.decode_attention_kv8(q[None].cuda(), codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), n, ws, sm_scale=sm)[0].cpu().double()
+    assert ws.status() == 0
+    vals = K8.values(codes, scales)
+    vs = 2.0 ** (scales[:, 1, 0, 0].double() - 127)
+    per_head = []
+    for h in range(Hq):
+        want, x, _, A, dot, U = K8.attention(q[h], vals[:, 0, 0, 0], vals[:, 1, 0, 0], sm, vs)
+        per_head.append((want, A, U, x, dot))
+    return o, per_head
+
+
+def _small_tolerance(want, A, U, x, dot, n, dtype):
+    """Half a step of the result; logits, weights and sums as for ordinary values; 32-bit intermediate results that are
+    subnormal are off by 2^-150 each, four to every pair of tiles, up to twice that after the division by the sum (>= 1/2)."""
+    de = 20 * 2.0 ** -23 * dot + 2.0 ** -22 * (2 + float(x.abs().max()) * LOG2E)
+    t = A * (2 * de + 2.0 ** -21 + (n / 4 + 32) * 2.0 ** -23) + 2.0 ** -38 * U + 8 * (n / 32 + 1) * 2.0 ** -150
+    return t + _half_step(want.abs() + t, dtype)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("Hq,D", [(4, 128), (12, 64)])
+@pytest.mark.parametrize("n", [5, 300, 3001])
+@pytest.mark.parametrize("low,high", [(-126, -120), (-118, -112), (-110, -100), (-126, -90)])
+def test_attention_over_the_smallest_values(T, dt, Hq, D, n, low, high):
+    """Value scales from 2^low to 2^high, down to the smallest there is: results are held down to the type's smallest."""
+    g = _gen(n + D - low)
+    codes = torch.randint(0, 256, (n, 2, 1, 1, D), generator=g).to(torch.uint8)
+    codes[codes & 127 == 127] = 0
+    scales = torch.full((n, 2, 1, 1), 121, dtype=torch.uint8)
+    scales[:, 1] = torch.randint(127 + low, 128 + high, (n, 1, 1), generator=g).to(torch.uint8)
+    q = (0.3 * torch.randn(Hq, D, generator=g)).to(DT[dt])
+    o, per_head = _attend_one(T, dt, q, codes, scales, n, 1 / math.sqrt(D))
+    assert o.abs().max() > 0
+    for h, (want, A, U, x, dot) in enumerate(per_head):
+        tol = _small_tolerance(want, A, U, x, dot, n, DT[dt])
+        assert ((o[h] - want).abs() <= tol).all(), (h, float(((o[h] - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n,heavy", [(70, 0), (300, 299), (1500, 700), (9000, 8999)])
+@pytest.mark.parametrize("logit", [70.0, 76.0, 84.0])
+def test_attention_behind_a_token_of_nearly_all_the_weight(T, dt, n, heavy, logit):
+    """The values of the heaviest token are zero, those of the others lie up to 121 binades of weight below it: the answer
+    is theirs."""
+    g = _gen(n)
+    D = 64
+    k, v = torch.zeros(n, 1, D), torch.randn(n, 1, D, generator=g)
+    k[heavy, 0, 0] = logit
+    v[heavy] = 0.0
+    kv, sc = T.alloc_kv8(n, 1, 1, D)
+    T.append_kv8(k.cuda(), v.cuda(), kv, sc)
+    q = torch.zeros(2, D)
+    q[:, 0] = 1.0
+    o, per_head = _attend_one(T, dt, q.to(DT[dt]), kv.cpu().view(torch.uint8), sc.cpu(), n, 1.0)
+    assert o.abs().max() > 0
+    for h, (want, A, U, x, dot) in enumerate(per_head):
+        # U counts the heaviest token's scale, which its values of zero do not use: 2^-126, out of account
+        tol = _small_tolerance(want, A, torch.zeros_like(U), x, dot, n, DT[dt])
+        assert ((o[h] - want).abs() <= tol).all(), float(((o[h] - want).abs() / tol).max())

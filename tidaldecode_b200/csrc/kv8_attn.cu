@@ -201,6 +201,18 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
+// 2^e as two factors, e an integer of at most 127.  One factor alone becomes zero below 2^-126, where the product with a sum
+// (up to 2^14 times as large as what it stands for) need not.
+struct Pow2 {
+    float a, b;
+    __device__ __forceinline__ explicit Pow2(float e) {
+        const int k = (int)fmaxf(e, -250.f), h = k >> 1;
+        a = __uint_as_float((uint32_t)(127 + h) << 23);
+        b = __uint_as_float((uint32_t)(127 + k - h) << 23);
+    }
+    __device__ __forceinline__ float times(float x) const { return x * a * b; }
+};
+
 // Softmax statistics and output of one query head to their final form.
 __device__ __forceinline__ float attn_kv8_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
 
@@ -647,7 +659,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                 if (head >= heads) continue;
-                const float f = fast_exp2(M[r][e] - m[r][e]) * (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f);
+                Pow2 f(M[r][e] - m[r][e]);
+                if (whole) f.b *= sum == 0.f ? 0.f : 1.f / sum;
                 const size_t out = row_of(cur.list) + head;
                 if (g == 0) {
                     if (!whole) *reinterpret_cast<float2*>(p.part_ml + (part + head) * 2) = make_float2(m[r][e], sum);
@@ -655,7 +668,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                 }
 #pragma unroll
                 for (int j = 0; j < KS; j += 2) {
-                    const float4 v = make_float4(o[r][j][e] * f, o[r][j][2 + e] * f, o[r][j + 1][e] * f, o[r][j + 1][2 + e] * f);
+                    const float4 v = make_float4(f.times(o[r][j][e]), f.times(o[r][j][2 + e]), f.times(o[r][j + 1][e]), f.times(o[r][j + 1][2 + e]));
                     if (whole) store4(reinterpret_cast<T*>(p.o) + out * D + g * VB + 2 * j, v);
                     else *reinterpret_cast<float4*>(p.part_o + (part + head) * D + g * VB + 2 * j) = v;
                 }
@@ -684,10 +697,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                 ml[warp][head][0] = m[r][e];
                 ml[warp][head][1] = sum;
             }
-            const float f = fast_exp2(M[r][e] - m[r][e]);
+            const Pow2 f(M[r][e] - m[r][e]);
             float* at = so + ((size_t)warp * p.rows + head) * D + g * VB;
 #pragma unroll
-            for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(o[r][j][e] * f, o[r][j][2 + e] * f);
+            for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(f.times(o[r][j][e]), f.times(o[r][j][2 + e]));
         }
     __syncthreads();
     for (int i = tid; i < heads * (D / 4); i += blockDim.x) {            // one unit to a CTA
@@ -698,13 +711,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         for (int w = 0; w < kKv8Warps; ++w) mx = fmaxf(mx, ml[w][head][0]);
 #pragma unroll
         for (int w = 0; w < kKv8Warps; ++w) {
-            const float f = fast_exp2(ml[w][head][0] - mx);
+            const Pow2 f(ml[w][head][0] - mx);
             const float4 v = *reinterpret_cast<const float4*>(so + ((size_t)w * p.rows + head) * D + d);
-            sum = fmaf(f, ml[w][head][1], sum);
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
+            sum += f.times(ml[w][head][1]);
+            acc.x = fmaf(f.a * v.x, f.b, acc.x);
+            acc.y = fmaf(f.a * v.y, f.b, acc.y);
+            acc.z = fmaf(f.a * v.z, f.b, acc.z);
+            acc.w = fmaf(f.a * v.w, f.b, acc.w);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const size_t out = row_of(cur.list) + head;
@@ -755,18 +768,18 @@ __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ 
     float mx = -FLT_MAX, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto rescale = [&](float to) {
-        const float f = fast_exp2(mx - to);
+        const Pow2 f(mx - to);
         mx = to;
-        sum *= f;
-        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+        sum = f.times(sum);
+        acc.x = f.times(acc.x), acc.y = f.times(acc.y), acc.z = f.times(acc.z), acc.w = f.times(acc.w);
     };
     auto add = [&](float m, float l, float4 v) {
-        const float f = fast_exp2(m - mx);
-        sum = fmaf(f, l, sum);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+        const Pow2 f(m - mx);
+        sum += f.times(l);
+        acc.x = fmaf(f.a * v.x, f.b, acc.x);
+        acc.y = fmaf(f.a * v.y, f.b, acc.y);
+        acc.z = fmaf(f.a * v.z, f.b, acc.z);
+        acc.w = fmaf(f.a * v.w, f.b, acc.w);
     };
     constexpr int K = 4;                                 // parts of a group in flight
     const int stride = split * groups;
