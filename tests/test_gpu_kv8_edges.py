@@ -192,3 +192,33 @@ def test_attention_behind_a_token_of_nearly_all_the_weight(T, dt, n, heavy, logi
         # U counts the heaviest token's scale, which its values of zero do not use: 2^-126, out of account
         tol = _small_tolerance(want, A, torch.zeros_like(U), x, dot, n, DT[dt])
         assert ((o[h] - want).abs() <= tol).all(), float(((o[h] - want).abs() / tol).max())
+
+
+# ----------------------------------------------- attention: tokens far below the heaviest
+@pytest.mark.parametrize("D,Hq", [(64, 1), (128, 1), (64, 12), (128, 12)])
+@pytest.mark.parametrize("n", [40, 300, 1000])
+@pytest.mark.parametrize("logit", [16.0, 18.0, 20.0, 26.0])
+def test_attention_keeps_the_bits_of_light_tokens(T, D, Hq, n, logit):
+    """fp32.  One token of ordinary values holds nearly all the weight, but half its elements are zero: there the answer is
+    what the other tokens carry, all of one weight 22 to 37 binades below, so that their roundings all go one way.  Off by
+    at most, of sum p|v|: 2^-20 the rounding of an exponential's argument (up to 64: half a step, times ln 2, is 2^-19 only
+    from 32 on), 2^-22 the exponential, 2^-22 a weight's two terms, 17 * 2^-24 a tile's product, 40 * 2^-24 the additions of a
+    warp's tiles and of the parts, 4 * 2^-24 the denominator and the division: less than 2^-17.  (A second term without a
+    factor of its own ends at 2^-24, 2^-38 of the heaviest weight: 2^-15 of a weight of 2^-24 of it, 2^-11 of 2^-28.)
+    And 2^-50 U: the second term goes in times 2^12, so its steps of 2^-24 stand for 2^-36 and it is off by 2^-37, where the
+    largest p_j 2^ev_j is scaled to more than 2^13; U = max_j (p_j 2^ev_j) * sum_j |code_j|."""
+    g = _gen(D + n)
+    k, v = torch.zeros(n, 1, D), torch.randn(n, 1, D, generator=g)
+    heavy = n // 3
+    k[:, 0, 0] = 0.34375
+    k[heavy, 0, 0] = logit
+    v[heavy, 0, :] = 1.0
+    v[heavy, 0, : D // 2] = 0.0
+    kv, sc = T.alloc_kv8(n, 1, 1, D)
+    T.append_kv8(k.cuda(), v.cuda(), kv, sc)
+    q = torch.zeros(Hq, D)
+    q[:, 0] = 1.0
+    o, per_head = _attend_one(T, "f32", q, kv.cpu().view(torch.uint8), sc.cpu(), n, 1.0)
+    for h, (want, A, U, x, dot) in enumerate(per_head):
+        off = ((o[h] - want).abs() / (2.0 ** -17 * A + 2.0 ** -50 * U)).max()
+        assert off <= 1, float(off)

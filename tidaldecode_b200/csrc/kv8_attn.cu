@@ -14,6 +14,10 @@
 // bits).  Weights are scaled to at most 2^14 (tokens down to 2^-38 of the heaviest still count) and enter the product as two
 // fp16 terms, the second the remainder of the first: one term alone (half a step is 2^-12) turned every fifteenth bf16 result
 // of a short list to the neighbouring number.  64 sequences of up to 32 K tokens, 32/8 heads of 128, bf16: 139 us, now 147.
+// Where the result is fp32 the remainder goes in times 2^12 and meets values times 2^-12 (e4m3 values are multiples of
+// 2^-9 of four bits: exact), so that its steps end 2^-50 below the heaviest weight in place of 2^-38: a weight has 22 bits
+// down to 2^-28 of it, where it had 11 (5 ragged sequences of up to 5 K tokens, 20/4 heads of 64: 12.9 us, now 13.1).  For
+// 16-bit results 11 bits at 2^-28 are enough, and the factors would cost 5 % of a long batch.
 // Accumulators, maxima and sums are fp32.  The tensor cores cut a sum's last bits off, and over a long chain that adds up (to
 // 8e-6 of a result after 30 K tokens, 1.7e-5 after 7 K tokens to a warp).  So where the result is fp32 the chain is short, and
 // what it gives is added by ordinary additions: after every tile where registers allow, after kKv8Chain tiles, with
@@ -125,10 +129,15 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The part of (lo, hi) that `packed` lost, again as fp16.
-__device__ __forceinline__ uint32_t pack_f16_rest(float lo, float hi, uint32_t packed) {
+// The part of (lo, hi) that `packed` lost, again as fp16, times `up`.
+__device__ __forceinline__ uint32_t pack_f16_rest(float lo, float hi, uint32_t packed, float up = 1.f) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
-    return pack_f16(lo - f.x, hi - f.y);
+    return pack_f16((lo - f.x) * up, (hi - f.y) * up);
+}
+// An fp16 pair times 2^-12, exact for e4m3 values: multiples of 2^-9 of four bits.
+__device__ __forceinline__ uint32_t shift_down(uint32_t x) {
+    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0x1p-12f));
+    return *reinterpret_cast<const uint32_t*>(&y);
 }
 
 __device__ __forceinline__ int list_len_kv8(const AttnKv8Params& p, int list) {
@@ -600,7 +609,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
                     pb[r][i] = transpose8x8(hi);
-                    pl[r][i] = transpose8x8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi));
+                    pl[r][i] = transpose8x8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi, QS ? 0x1p12f : 1.f));
                 }
             }
             // ---- O^T += V^T P^T
@@ -625,20 +634,26 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                     halves_of(__byte_perm(vw[2 * h2][w], vw[2 * h2 + 1][w], 0x7362), a[h2][2], a[h2][3]);
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t low[4] = {a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1]};      // operand of the second terms
+                    if (QS) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) low[i] = shift_down(low[i]);
+                    }
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
                         if (QS && !park) {
                             float part[4];
-                            mma_f16_fresh(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[r][0], pl[r][1]);
+                            mma_f16_fresh(part, low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
                             mma_f16(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[r][2 * w + e][i] += part[i];
                             continue;
                         }
                         mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
-                        mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pl[r][0], pl[r][1]);
+                        mma_f16(o[r][2 * w + e], low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
                     }
+                }
             }
         }
         if (looked) park_scales(ahead >> 1);
