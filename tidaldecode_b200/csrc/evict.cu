@@ -222,10 +222,11 @@ constexpr int kEvictKeys = 47 * 1024;     // page keys a CTA keeps in shared mem
 __global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[3][kEvictBins];
+    __shared__ uint2 hist2[3][kEvictBins / 2];                   // read in pairs: by type on 8 bytes
     __shared__ uint32_t few[kEvictFew];
     __shared__ int sums[32], s_pick[3], s_ties, s_more, s_few;
     __shared__ int warp_ties[32], warp_more[32];
+    uint32_t (*const hist)[kEvictBins] = reinterpret_cast<uint32_t (*)[kEvictBins]>(hist2);
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_pages_kernel(const EvictP
             const int bin = kEvictBins - 2 - 2 * tid;
             int c0 = 0, c1 = 0;
             for (int r = 0; r < C; ++r) {
-                const uint2 v = *reinterpret_cast<const uint2*>((C > 1 ? cluster.map_shared_rank(&hist[d][0], r) : &hist[d][0]) + bin);
+                const uint2 v = (C > 1 ? cluster.map_shared_rank(&hist2[d][0], r) : &hist2[d][0])[bin / 2];
                 c0 += (int)v.x;
                 c1 += (int)v.y;
             }

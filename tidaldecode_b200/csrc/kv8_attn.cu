@@ -205,7 +205,7 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     if (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(p) = v;
     } else {
-        const T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+        alignas(8) const T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
         *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
     }
 }
@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ AttnKv8Params p, int split) {
     extern __shared__ int prefix_m[];                    // [lists + 1], ragged
-    __shared__ float sh_o[8][D];
+    __shared__ float4 sh_o[8][D / 4];                    // by type on 16 bytes
     __shared__ float sh_ml[8][2];
     __shared__ int s_scan[8];
     if (threadIdx.x == 0) TIDAL_STAMP(8);
@@ -826,13 +826,13 @@ __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ 
         acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
     }
     if (split > 1) {
-        if (place == 0) *reinterpret_cast<float4*>(&sh_o[warp][chunk * 32 + d]) = acc;
+        if (place == 0) sh_o[warp][(chunk * 32 + d) / 4] = acc;
         if (lane == 0) sh_ml[warp][0] = mx, sh_ml[warp][1] = sum;
         __syncthreads();
         if (member == 0 && place == 0) {
             for (int w = 1; w < split; ++w) top = fmaxf(top, sh_ml[warp + w][0]);
             rescale(top);
-            for (int w = 1; w < split; ++w) add(sh_ml[warp + w][0], sh_ml[warp + w][1], *reinterpret_cast<const float4*>(&sh_o[warp + w][chunk * 32 + d]));
+            for (int w = 1; w < split; ++w) add(sh_ml[warp + w][0], sh_ml[warp + w][1], sh_o[warp + w][(chunk * 32 + d) / 4]);
         }
     }
     if (work && member == 0 && place == 0) {
