@@ -1,0 +1,45 @@
+"""What stands beside a bounded cache: Quest metadata that follow the cache, generation that runs on, eviction that has
+something to go by."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import tidal_oracle as O
+from tests.test_gpu_kv8_model import _controller
+from tests.test_gpu_model import _tiny_model
+
+pytestmark = pytest.mark.gpu
+
+
+def _estimates_are_the_keys(c, U, q, layers, stored):
+    """Pages hold one token, so the bound of a page is the token's logit itself: 64 products and their sum in 32 bits."""
+    for layer in layers:
+        got = U.decode_estimate(q, c, layer).cpu().double()
+        keys = stored[layer][:got.shape[1]]                                          # [n - 1, Hkv, D]
+        for h in range(q.shape[1]):
+            terms = keys[:, h // 4].double() * q[0, h].cpu().double()
+            assert ((got[h] - terms.sum(1)).abs() <= 64 * 2.0 ** -24 * terms.abs().sum(1)).all(), (layer, h)
+
+
+def _in_order(c, layer):
+    """The cached keys of sequence 0 in slot order."""
+    pages = torch.tensor(c.kv_cache._indicies[0][:c.kv_cache.seqlen])
+    return c.kv_cache.buf_layer(layer)[pages.cuda(), 0, 0].cpu()
+
+
+@pytest.mark.parametrize("layer_alias", [1, 2])
+def test_quest_metadata_of_a_controller(layer_alias):
+    """append_kv keeps the per-page key bounds, decode_estimate reads them, per layer (or per pool that layers share)."""
+    import tidaldecode_b200.utils as U
+    g = torch.Generator().manual_seed(1)
+    n = 70
+    c = _controller(16, False, dtype=torch.float32, quest_metadata=True, layer_alias=layer_alias)
+    for new in (n, 1, 1):
+        c.prepare_metadata(new)
+        c.begin_forward(new)
+        for layer in range(2):
+            k, v = (torch.randn(new, 2, 64, generator=g).cuda() for _ in range(2))
+            U.append_kv(k, v, c, layer)
+    q = torch.randn(1, 8, 64, generator=g).cuda()
+    _estimates_are_the_keys(c, U, q, range(2), [_in_order(c, layer) for layer in range(2)])

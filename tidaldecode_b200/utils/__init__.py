@@ -83,7 +83,7 @@ def _update_quest_metadata(c: InferenceController, layer_idx: int, new_tokens: i
     if c.metadata_cache is None:
         return
     n = c.kv_cache.seqlen
-    ops.update_page_meta(c.kv_cache.buf_layer(layer_idx), c.metadata_cache[layer_idx // c.kv_cache.layer_alias], n, n - new_tokens,
+    ops.update_page_meta(c.kv_cache.buf_layer(layer_idx), c.metadata_layer(layer_idx), n, n - new_tokens,
                          batch=c.batch_size, page_table=c.kv_cache.page_table, meta_pages_per_seq=c.metadata_cache.shape[1] // c.batch_size)
 
 
@@ -112,7 +112,7 @@ def decode_estimate(q: torch.Tensor, iController: InferenceController, layer_idx
         raise RuntimeError("decode_estimate needs InferenceController(..., quest_metadata=True)")
     n = c.kv_cache.num_pages - 1
     o = torch.empty(q.shape[1], max(n, 1), dtype=q.dtype, device=q.device)
-    ops.estimate(q[:1].contiguous(), c.metadata_cache[layer_idx // c.kv_cache.layer_alias], n, out=o.view(1, *o.shape),
+    ops.estimate(q[:1].contiguous(), c.metadata_layer(layer_idx), n, out=o.view(1, *o.shape),
                  meta_pages_per_seq=c.metadata_cache.shape[1] // c.batch_size)
     return o[:, :n]
 

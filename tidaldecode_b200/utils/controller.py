@@ -122,6 +122,10 @@ class InferenceController:
         self.prefill_latency = []
         self.decode_latency = []
 
+    def metadata_layer(self, layer_idx: int) -> torch.Tensor:
+        """Quest metadata of the pool that `kv_cache.buf_layer(layer_idx)` is (layers that share the one share the other)."""
+        return self.metadata_cache[layer_idx % self.kv_cache.pool.num_layers]
+
     # Used for controlling the number of pages (reference: skips the first layers by raising it)
     def set_token_budget(self, token_budget: int):
         self._token_budget = token_budget
