@@ -43,3 +43,31 @@ def test_quest_metadata_of_a_controller(layer_alias):
             U.append_kv(k, v, c, layer)
     q = torch.randn(1, 8, 64, generator=g).cuda()
     _estimates_are_the_keys(c, U, q, range(2), [_in_order(c, layer) for layer in range(2)])
+
+
+@pytest.mark.parametrize("layer_alias", [1, 2])
+def test_quest_metadata_follow_an_eviction(layer_alias):
+    """After slots have been renumbered a page's bounds are those of the token it holds now, in every layer; so are those of
+    the tokens appended next."""
+    import tidaldecode_b200.utils as U
+    g = torch.Generator().manual_seed(2)
+    n, keep = 90, 40
+    c = _controller(16, True, dtype=torch.float32, quest_metadata=True, layer_alias=layer_alias)
+    q = torch.randn(1, 8, 64, generator=g).cuda()
+
+    def append(new):
+        c.prepare_metadata(new)
+        c.begin_forward(new)
+        for layer in range(2):
+            k, v = (torch.randn(new, 2, 64, generator=g).cuda() for _ in range(2))
+            U.append_kv(k, v, c, layer)
+
+    append(n)
+    append(1)
+    U.decode_sparse_attn(q, c, 0, c.kv_indices_without_last, True)
+    before = c.kv_cache._indicies[0][:n + 1]
+    assert U.evict_kv(c, keep, 2, 5) == n + 1 - keep and c.kv_cache._indicies[0][:keep] != before[:keep]
+    _estimates_are_the_keys(c, U, q, range(2), [_in_order(c, layer) for layer in range(2)])
+    append(1)
+    append(1)
+    _estimates_are_the_keys(c, U, q, range(2), [_in_order(c, layer) for layer in range(2)])

@@ -201,4 +201,8 @@ def evict_kv(iController: InferenceController, keep_tokens: int, sink_tokens: in
     if c.weights is None:
         raise RuntimeError("evict_kv needs InferenceController(..., track_weights=True)")
     c._selection_valid = False
-    return c.kv_cache.evict(c.weights, keep_tokens, sink_tokens, recent_tokens)
+    dropped = c.kv_cache.evict(c.weights, keep_tokens, sink_tokens, recent_tokens)
+    if dropped and c.metadata_cache is not None:                 # key bounds lie by slot: the slots have been renumbered
+        for layer in range(c.kv_cache.pool.num_layers):
+            _update_quest_metadata(c, layer, c.kv_cache.seqlen)
+    return dropped
