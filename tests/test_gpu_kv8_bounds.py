@@ -71,3 +71,33 @@ def test_quest_metadata_follow_an_eviction(layer_alias):
     append(1)
     append(1)
     _estimates_are_the_keys(c, U, q, range(2), [_in_order(c, layer) for layer in range(2)])
+
+
+def test_a_bounded_cache_generates_without_end():
+    """170 tokens through a cache of 96, with evictions between the calls: replayed, eager and in calls of one token the same
+    tokens, and what earlier calls returned stays as it was."""
+    from tidaldecode_b200.runtime import GraphDecoder
+    W = O.TinyLlamaWeights(vocab=512, hidden=512, layers=4, heads=8, kv_heads=2, ffn=352, seed=5, dtype=torch.bfloat16)
+    prompt = torch.randint(0, 512, (1, 60), generator=torch.Generator().manual_seed(3))
+    runs = []
+    for use_graph, at_once in ((True, True), (False, True), (True, False)):
+        rt = GraphDecoder(_tiny_model(W, torch.bfloat16, (1, 3), "none", True, 2), max_seq_len=96, token_budget=16, kv_bits=8, track_weights=True)
+        rt.prefill(prompt)
+        parts, copies = [], []
+        for steps in (20, 50, 50, 50):
+            got = [rt.decode(steps, use_graph=use_graph)] if at_once else [rt.decode(1, use_graph=use_graph) for _ in range(steps)]
+            assert torch.equal(got[-1][:, -1:], rt.tok)
+            parts += got
+            copies += [x.clone() for x in got]
+            rt.evict(40, sink_tokens=2, recent_tokens=8)
+            assert rt.c.kv_cache.seqlen == 40
+        assert int(rt.pos) == 60 + 170 and int(rt.slot) == 40 and rt.c.workspace.status() == 0 and int(rt.lin_status) == 0
+        with pytest.raises(RuntimeError, match="max_seq_len"):
+            rt.decode(57, use_graph=use_graph)
+        assert all(torch.equal(a, b) for a, b in zip(parts, copies))
+        runs.append(torch.cat(parts, 1))
+        assert runs[-1].shape == (1, 170)
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    # a new conversation starts over
+    rt.prefill(prompt)
+    assert torch.equal(rt.decode(20), runs[0][:, :20])

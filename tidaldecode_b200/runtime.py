@@ -56,6 +56,7 @@ class GraphDecoder:
         self.pos = torch.zeros(self.B, **i32)               # its position
         self.slot = torch.zeros(self.B, **i32)              # its cache slot: the position less the tokens evicted (8-bit cache)
         self._evicted = self._done = 0                      # tokens dropped and decoded since the prompt
+        self._column = 0                                    # of out_tokens that the next decode() call writes first
         self.row_lens = torch.zeros(self.rows, **i32)       # seq_lens per score row
         self.sel_counts = torch.zeros(self.rows, **i32)
         self.tok = torch.zeros(self.B, 1, dtype=torch.int64, device=self.device)
@@ -99,7 +100,7 @@ class GraphDecoder:
         self.seq_lens.fill_(P + 1)
         self.pos.fill_(P)
         self.slot.fill_(P)
-        self._evicted = self._done = 0
+        self._evicted = self._done = self._column = 0
         self.row_lens.fill_(P + 1)
         self.tok.copy_(first.view(self.B, 1))
         self.step_idx.zero_()
@@ -122,7 +123,7 @@ class GraphDecoder:
         self.seq_lens.fill_(seq_len + 1)
         self.pos.fill_(seq_len)
         self.slot.fill_(seq_len)
-        self._evicted = self._done = 0
+        self._evicted = self._done = self._column = 0
         self.row_lens.fill_(seq_len + 1)
         self.tok.copy_(first_tokens.view(self.B, 1).to(self.device))
         self.step_idx.zero_()
@@ -221,11 +222,15 @@ class GraphDecoder:
     @torch.inference_mode()
     def decode(self, steps: int, use_graph: bool = True) -> torch.Tensor:
         """`steps` more greedy tokens (the first call continues after the token `prefill` returned);
-        returns those `steps` tokens, [B, steps] on the device."""
+        returns those `steps` tokens, [B, steps] on the device.  The cache holds max_seq_len tokens; with evictions
+        between calls generation has no end of its own."""
         asked = steps
         held = self._prefill_len - self._evicted               # tokens of the prompt's account still in the cache
-        if held + max(1, self._done) + steps > self.max_seq_len or self._done + steps > self.out_tokens.shape[1]:
+        if held + max(1, self._done) + steps > self.max_seq_len:
             raise RuntimeError("max_seq_len too small for this many steps")
+        if self._column + steps > self.out_tokens.shape[1]:    # a cache that evictions keep bounded runs on: columns are used again
+            self.step_idx.zero_()
+            self._column = 0
         if not use_graph:
             for _ in range(steps):
                 self._step()
@@ -242,9 +247,11 @@ class GraphDecoder:
                 # the capture pass does not execute: nothing to undo
             for _ in range(steps):
                 self.graph.replay()
-        done = self._done = int(self.step_idx.item())
-        self.c.kv_cache._seqlen = self._prefill_len + done - self._evicted      # host bookkeeping catches up with the device
-        return self.out_tokens[:, done - asked:done]
+        end = int(self.step_idx.item())
+        self._done += end - self._column
+        self._column = end
+        self.c.kv_cache._seqlen = self._prefill_len + self._done - self._evicted      # host bookkeeping catches up with the device
+        return self.out_tokens[:, end - asked:end].clone()
 
     def evict(self, keep_tokens: int, sink_tokens: int = 4, recent_tokens: int = 64) -> int:
         """Between two decode() calls: drop the cached tokens that the selection layers have attended to least until
