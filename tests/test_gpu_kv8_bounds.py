@@ -101,3 +101,31 @@ def test_a_bounded_cache_generates_without_end():
     # a new conversation starts over
     rt.prefill(prompt)
     assert torch.equal(rt.decode(20), runs[0][:, :20])
+
+
+def test_eviction_needs_weights():
+    """Straight after a prompt no token has a weight: dropping "the lightest" is refused and changes nothing, while the first
+    and the last tokens alone can be kept, and a cache within its budget is left alone."""
+    import tidaldecode_b200.utils as U
+    g = torch.Generator().manual_seed(4)
+    c = _controller(8, True, B=2)
+    c.prepare_metadata(100)
+    c.begin_forward(100)
+    k, v = (torch.randn(200, 2, 64, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    U.append_kv(k, v, c, 0)
+    pages = [list(x) for x in c.kv_cache._indicies]
+    with pytest.raises(RuntimeError, match="attention weights"):
+        U.evict_kv(c, 50, 4, 10)
+    assert c.kv_cache.seqlen == 100 and c.kv_cache._indicies == pages and c.kv_cache.pos_base == 0
+    assert U.evict_kv(c, 100, 4, 10) == 0
+    assert U.evict_kv(c, 50, 10, 40) == 50
+    assert [x[:50] for x in c.kv_cache._indicies] == [x[:10] + x[60:] for x in pages]
+    c.prepare_metadata(1)
+    c.begin_forward(1)
+    U.append_kv(k[:2], v[:2], c, 0)
+    U.decode_sparse_attn(torch.randn(2, 8, 64, generator=g).to(torch.bfloat16).cuda(), c, 0, c.kv_indices_without_last, True)
+    assert U.evict_kv(c, 40, 4, 10) == 11
+    c.clean_states()
+    c.prepare_metadata(100)
+    with pytest.raises(RuntimeError, match="attention weights"):
+        U.evict_kv(c, 50, 4, 10)

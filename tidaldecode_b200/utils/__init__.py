@@ -195,11 +195,17 @@ def _decode_attn_kv8(q, o, c: InferenceController, layer_idx: int, topk_indices:
 def evict_kv(iController: InferenceController, keep_tokens: int, sink_tokens: int = 4, recent_tokens: int = 64) -> int:
     """Bound the cache between two steps: of every sequence the first sink_tokens, the last recent_tokens and those that the
     selection layers' queries have attended to most stay, keep_tokens in all; returns the tokens dropped per sequence.
-    Needs a controller built with track_weights=True.  Positions go on counting (later queries and keys are rotated as
+    Needs a controller built with track_weights=True and, where tokens compete (keep_tokens above sink plus recent),
+    at least one decode step through a selection layer since clean_states(): a prompt's own attention is not added up,
+    and with all weights zero there is nothing to rank by.  Positions go on counting (later queries and keys are rotated as
     if nothing had been dropped); the set of the last selection is forgotten.  No reference counterpart."""
     c = iController
     if c.weights is None:
         raise RuntimeError("evict_kv needs InferenceController(..., track_weights=True)")
+    n = c.kv_cache.seqlen
+    if sink_tokens + max(1, recent_tokens) < keep_tokens < n and not bool((c.weights[:, :n] != 0).any(1).all()):
+        raise RuntimeError("evict_kv: no selection layer has added attention weights yet (decode a few steps first, or keep "
+                           "no more than sink_tokens + recent_tokens)")
     c._selection_valid = False
     dropped = c.kv_cache.evict(c.weights, keep_tokens, sink_tokens, recent_tokens)
     if dropped and c.metadata_cache is not None:                 # key bounds lie by slot: the slots have been renumbered
