@@ -471,8 +471,8 @@ typedef struct {
 int tidal_append_kv8(const tidal_append_kv8_args* args, void* stream);
 
 /* Slots [start, stop) of every sequence of an 8-bit pool as rows of dtype: d_out [batch][stop - start][2][Hkv][D] — per
- * sequence a 16/32-bit pool of page_size 1, as tidal_prefill takes it.  f16 saturates at +-65504.  With d_seq_lens,
- * rows at and behind a sequence's length are left as they were; so are rows whose page lies outside the pool
+ * sequence a 16/32-bit pool of page_size 1, as tidal_prefill takes it.  Values beyond the type's largest saturate.
+ * With d_seq_lens, rows at and behind a sequence's length are left as they were; so are rows whose page lies outside the pool
  * (TIDAL_DEV_BAD_INDEX in *d_status). */
 typedef struct {
     const void* d_kv;

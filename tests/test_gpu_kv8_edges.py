@@ -222,3 +222,19 @@ def test_attention_keeps_the_bits_of_light_tokens(T, D, Hq, n, logit):
     for h, (want, A, U, x, dot) in enumerate(per_head):
         off = ((o[h] - want).abs() / (2.0 ** -17 * A + 2.0 ** -50 * U)).max()
         assert off <= 1, float(off)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+def test_read_over_all_scales_and_codes(T, dt):
+    """Every code at every scale from zero and 2^-126 to 2^120: one rounding to the type, and what lies beyond its largest
+    number saturates (32 bits hold every value but those of 2^128 and more, which codes from 256 on have at scale 2^120:
+    the largest finite floats are stored so)."""
+    n, D = 248, 128
+    codes = torch.arange(256).view(1, 2, 1, 1, D).expand(n, 2, 1, 1, D).to(torch.uint8).contiguous()
+    scales = torch.arange(n).view(n, 1, 1, 1).expand(n, 2, 1, 1).to(torch.uint8).contiguous()
+    got = T.read_kv8(codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), n, dtype=DT[dt])[0, :, :, 0, 0].cpu()
+    want = K8.values(codes, scales)[:, :, 0, 0]
+    assert torch.equal(want[:247].float().double().nan_to_num(), want[:247].nan_to_num())
+    most = torch.finfo(DT[dt]).max
+    want = want.float().clamp(-most, most).to(DT[dt])
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~torch.isnan(got)], want[~torch.isnan(want)])

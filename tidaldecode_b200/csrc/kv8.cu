@@ -1,5 +1,6 @@
 // Writing and reading an 8-bit KV pool: quantised append of new tokens, and read-back as 16/32-bit rows.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -286,9 +287,12 @@ __global__ void __launch_bounds__(256) read_kv8_kernel(const ReadKv8Params p) {
         values8(make_uint2(c[s].x, c[s].y), x);
         values8(make_uint2(c[s].z, c[s].w), x + 8);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] *= k;
-            if (std::is_same<T, __half>::value) x[i] = x[i] > 65504.f ? 65504.f : (x[i] < -65504.f ? -65504.f : x[i]);
+        for (int i = 0; i < 16; ++i) x[i] *= k;
+        // 2^120, the scale of the largest floats, is the one at which 32-bit and bf16 rows can pass their type's end
+        if (std::is_same<T, __half>::value || sc[s] >= 247u) {
+            constexpr float most = std::is_same<T, __half>::value ? 65504.f : sizeof(T) == 4 ? FLT_MAX : 0x1.fep127f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = x[i] > most ? most : (x[i] < -most ? -most : x[i]);
         }
 #pragma unroll
         for (int i = 0; i < 16; i += V::N) to[i / V::N] = V::from_float(x + i);
