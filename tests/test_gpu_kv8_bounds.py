@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from oracle import kv8_oracle as K8
 from oracle import tidal_oracle as O
 from tests.test_gpu_kv8_model import _controller
 from tests.test_gpu_model import _tiny_model
@@ -129,3 +130,48 @@ def test_eviction_needs_weights():
     c.prepare_metadata(100)
     with pytest.raises(RuntimeError, match="attention weights"):
         U.evict_kv(c, 50, 4, 10)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kv_bits", [8, 16])
+def test_selection_layer_with_weights_against_its_definition(kv_bits, dtype):
+    """With track_weights a selection layer's output, logits, log-sum-exp and weights are those of its definition over the
+    cached values.  Logits: 128 roundings of fp32 sums of |q k| at most (64 products, any order, the scale).  Weights and
+    output follow with twice their error, the output with half a step of its type and of the softmax weights' type."""
+    import math
+    import tidaldecode_b200.utils as U
+    g = torch.Generator().manual_seed(6)
+    B, n = 2, 180
+    c = _controller(kv_bits, True, dtype=dtype, B=B)
+    k, v = (torch.randn(B * n, 2, 64, generator=g).to(dtype).cuda() for _ in range(2))
+    c.prepare_metadata(n)
+    U.append_kv(k, v, c, 0)
+    c.prepare_metadata(1)
+    c.begin_forward(1)
+    U.append_kv(k[:B], v[:B], c, 0)
+    q = torch.randn(B, 8, 64, generator=g).to(dtype).cuda()
+    o = U.decode_sparse_attn(q, c, 0, c.kv_indices_without_last, True)
+    n += 1
+    eps = torch.finfo(dtype).eps / 2
+    for b in range(B):
+        rows = c.kv_cache.buf_layer(0)[torch.tensor(c.kv_cache._indicies[b][:n]).cuda()]
+        if kv_bits == 8:
+            scales = c.kv_cache.scales_layer(0)[torch.tensor(c.kv_cache._indicies[b][:n]).cuda()]
+            rows = K8.values(rows.cpu(), scales.cpu()).cuda()
+        K, V = rows[:, 0, 0].double(), rows[:, 1, 0].double()                       # [n, Hkv, D]
+        weights = torch.zeros(n, dtype=torch.float64, device="cuda")
+        far = 0.0
+        for h in range(8):
+            kk, vv = K[:, h // 4], V[:, h // 4]
+            x = kk @ q[b, h].double() / 8
+            dx = 128 * 2.0 ** -24 * float((kk.abs() @ q[b, h].double().abs()).max()) / 8 + 2.0 ** -22 * (2 + float(x.abs().max()) * 1.4427)
+            z = x.logsumexp(0)
+            p = torch.exp(x - z)
+            assert (c.qk_product[b, h, :n].double() - x).abs().max() <= dx
+            assert abs(float(c.lse[b, h]) - float(z)) <= dx + (n + 8) * 2.0 ** -24 + 2.0 ** -22 * abs(float(z))
+            A = p @ vv.abs()
+            assert ((o[b, h].double() - p @ vv).abs() <= eps * (p @ vv).abs() + A * (2 * dx + (eps if dtype != torch.float32 else 0) + (n + 32) * 2.0 ** -23)).all()
+            weights += p
+            far = max(far, dx)
+        assert ((c.weights[b, :n].double() - weights).abs() <= weights * (2 * far + (n + 16) * 2.0 ** -23)).all()
+    assert c.workspace.status() == 0 and not c.weights[:, n:].any()

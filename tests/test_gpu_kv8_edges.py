@@ -238,3 +238,42 @@ def test_read_over_all_scales_and_codes(T, dt):
     most = torch.finfo(DT[dt]).max
     want = want.float().clamp(-most, most).to(DT[dt])
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~torch.isnan(got)], want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("Hq,D", [(1, 64), (8, 64), (8, 128), (12, 128)])
+def test_attention_long_sums_of_ordinary_weights(T, Hq, D):
+    """fp32, 20 000 tokens, many to a warp, ordinary softmax weights and values of both signs, in the root mean square of a
+    result.  Queries and keys are few multiples of powers of two: the products' sums are exact.  What is left:
+        2^-20.5   the argument of an exponential, below 32: half a step of 2^-19 times ln 2
+        2^-22     the exponential; 2^-22 a weight's two terms; 2^-22 the merge and the division
+        E         the common factor of all logits, sm log2 e, off by 2^-23 of itself: moves a weight by 2^-23 ln 2 (x - mean x)
+        2 sqrt(n/16)/3 * 2^-24     additions rounded to nearest, as for equal weights."""
+    g = _gen(D + Hq)
+    n, page, B, sm = 20000, 16, 300, 2.0 ** -4 if D == 128 else 2.0 ** -3.5
+    sm = float(torch.tensor(sm, dtype=torch.float32))
+    k = torch.randint(-8, 9, (n, 1, D), generator=g) * 0.25
+    codes = torch.randint(0, 256, (n // page, 2, page, 1, D), generator=g).to(torch.uint8)
+    codes[codes & 127 == 127] = 0
+    codes[:, 0] = k.to(torch.float8_e4m3fn).view(torch.uint8).view(n // page, page, 1, D)
+    scales = torch.full((n // page, 2, 1, 1), 120, dtype=torch.uint8)
+    scales[:, 0] = 127
+    q = torch.randint(-8, 9, (B, Hq, D), generator=g) / 4.0
+    ws = T.Workspace(B, Hq, D, 1, 1)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(B, -1).contiguous()
+    o = T.decode_attention_kv8(q.cuda(), codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), n, ws, page_table=table, sm_scale=sm).double()
+    assert ws.status() == 0
+    vals = K8.values(codes, scales).cuda()
+    K, V = vals[:, 0, :, 0].reshape(n, D), vals[:, 1, :, 0].reshape(n, D)
+    assert torch.equal(K.cpu(), k[:, 0].double())
+    worst = 0.0
+    for b in range(0, B, 20):
+        x = q[b:b + 20].cuda().double().view(-1, D) @ K.T * sm
+        p = torch.softmax(x, 1)
+        want = p @ V
+        assert (x.amax(1) - x.amin(1)).max() * LOG2E + 1 < 32
+        factor = (p * (x - (p * x).sum(1, keepdim=True))) @ V * 2.0 ** -23
+        size = want.norm(dim=1)
+        tol = 2.0 ** -20.5 + 3 * 2.0 ** -22 + factor.norm(dim=1) / size + 2 * math.sqrt(n / 16) / 3 * 2.0 ** -24
+        off = (o[b:b + 20].view(-1, D) - want).norm(dim=1) / size
+        worst = max(worst, float((off / tol).max()))
+    assert worst <= 1, worst
