@@ -33,7 +33,7 @@ def _half_step(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 # --------------------------------------------------------------- attention: last bits
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
-@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 12, 1), (128, 16, 1)])
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 12, 1), (128, 16, 1), (128, 8, 1), (64, 7, 1), (64, 6, 2), (128, 3, 3)])
 def test_attention_rounds_16_bit_results_once(T, dt, D, Hq, Hkv):
     """A 16-bit result is the 64-bit one rounded to its type: off by half a step and by what 32-bit arithmetic loses.  The
     softmax weights have no rounding of their own beyond that: held in two fp16 terms they are off by 2^-22.  With
@@ -153,7 +153,7 @@ def _small_tolerance(want, A, U, x, dot, n, dtype):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
-@pytest.mark.parametrize("Hq,D", [(4, 128), (12, 64)])
+@pytest.mark.parametrize("Hq,D", [(4, 128), (12, 64), (2, 64), (7, 128)])
 @pytest.mark.parametrize("n", [5, 300, 3001])
 @pytest.mark.parametrize("low,high", [(-126, -120), (-118, -112), (-110, -100), (-126, -90)])
 def test_attention_over_the_smallest_values(T, dt, Hq, D, n, low, high):
@@ -195,7 +195,7 @@ def test_attention_behind_a_token_of_nearly_all_the_weight(T, dt, n, heavy, logi
 
 
 # ----------------------------------------------- attention: tokens far below the heaviest
-@pytest.mark.parametrize("D,Hq", [(64, 1), (128, 1), (64, 12), (128, 12)])
+@pytest.mark.parametrize("D,Hq", [(64, 1), (128, 1), (64, 12), (128, 12), (64, 4), (128, 3), (64, 8), (128, 5)])
 @pytest.mark.parametrize("n", [40, 300, 1000])
 @pytest.mark.parametrize("logit", [16.0, 18.0, 20.0, 26.0])
 def test_attention_keeps_the_bits_of_light_tokens(T, D, Hq, n, logit):
@@ -240,7 +240,7 @@ def test_read_over_all_scales_and_codes(T, dt):
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~torch.isnan(got)], want[~torch.isnan(want)])
 
 
-@pytest.mark.parametrize("Hq,D", [(1, 64), (8, 64), (8, 128), (12, 128)])
+@pytest.mark.parametrize("Hq,D", [(1, 64), (8, 64), (8, 128), (12, 128), (4, 64), (3, 128)])
 def test_attention_long_sums_of_ordinary_weights(T, Hq, D):
     """fp32, 20 000 tokens, many to a warp, ordinary softmax weights and values of both signs, in the root mean square of a
     result.  Queries and keys are few multiples of powers of two: the products' sums are exact.  What is left:

@@ -11,13 +11,15 @@
 //
 // Rounding choices.  q is scaled by a power of two so that its largest element lies in [2^11, 2^12): fp16 then holds
 // bf16 and fp16 rows exactly (elements 2^25 below the largest lose bits); fp32 rows are split into two fp16 terms (22
-// bits).  Weights are scaled to at most 2^14 (tokens down to 2^-38 of the heaviest still count) and enter the product as two
-// fp16 terms, the second the remainder of the first: one term alone (half a step is 2^-12) turned every fifteenth bf16 result
-// of a short list to the neighbouring number.  64 sequences of up to 32 K tokens, 32/8 heads of 128, bf16: 139 us, now 147.
-// Where the result is fp32 the remainder goes in times 2^12 and meets values times 2^-12 (e4m3 values are multiples of
-// 2^-9 of four bits: exact), so that its steps end 2^-50 below the heaviest weight in place of 2^-38: a weight has 22 bits
-// down to 2^-28 of it, where it had 11 (5 ragged sequences of up to 5 K tokens, 20/4 heads of 64: 12.9 us, now 13.1).  For
-// 16-bit results 11 bits at 2^-28 are enough, and the factors would cost 5 % of a long batch.
+// bits).  Weights are scaled to at most 2^14 and enter the product as two fp16 terms, the second the remainder of the first: one
+// term alone (half a step is 2^-12) turned every fifteenth bf16 result of a short list to the neighbouring number.  Up to
+// four query heads to a unit leave half of the product's eight columns free: they hold the second terms (the free columns
+// mirror the queries, so that a lane forms a remainder from logits of its own), times 2^12, and the sums are joined when the
+// list ends.  A weight then has 22 bits down to 2^-28 of the heaviest, and tokens down to 2^-50 of it count.  With more
+// heads the second terms are a product of their own: for fp32 results times 2^12 as well, against values times 2^-12 (e4m3
+// values are multiples of 2^-9 of four bits: exact); for 16-bit results as they are, 11 bits at 2^-28 and an end at 2^-38,
+// which such results do not show and which saves 5 % of a long batch.  64 sequences of up to 32 K tokens, 32/8 heads of 128,
+// bf16: 138 us with one term, 148 with a second product, 142 with the columns.
 // Accumulators, maxima and sums are fp32.  The tensor cores cut a sum's last bits off, and over a long chain that adds up (to
 // 8e-6 of a result after 30 K tokens, 1.7e-5 after 7 K tokens to a warp).  So where the result is fp32 the chain is short, and
 // what it gives is added by ordinary additions: after every tile where registers allow, after kKv8Chain tiles, with
@@ -235,9 +237,9 @@ __device__ __forceinline__ int range_of(int i, int total, int ranges) { return (
 // warp; where a list is shared, each leaves a partial (o relative to m, m, l) and merge_kv8_kernel adds them in order.
 // The order of additions depends on the lengths and the launch alone.  Short lists go the other way (solo): one CTA per
 // list and unit, whose warps merge through shared memory, with no second launch.
-template <typename T, int D, bool R2>    // R2: more than 8 query heads to a unit
-__global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 128) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
-    constexpr bool QS = sizeof(T) == 4;
+template <typename T, int D, int H>      // H: query heads to a unit, at most: 4, 8 or 16
+__global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || D == 128) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
+    constexpr bool QS = sizeof(T) == 4, R2 = H == 16, MIRROR = H == 4;
     constexpr int S = Kv8Ring<D, R2>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
     constexpr bool park = QS && D == 128 && !R2;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -420,6 +422,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 #pragma unroll
         for (int i = 0; i < NR * KS * 4; ++i) o[i / (4 * KS)][i / 4 % KS][i % 4] += parked[i];
     };
+    // MIRROR: what the second terms gave, in the columns of heads 4 to 7, is added to the first terms' sums
+    auto fold = [&]() {
+        if (!MIRROR) return;
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[0][j][i] = fmaf(__shfl_xor_sync(0xffffffffu, o[0][j][i], 2), 0x1p-12f, o[0][j][i]);
+    };
     for (int it = 0; it < n_it || (p.solo && fresh); ++it) {
         const int ahead = it + S - 1;
         const bool looked = ahead < n_it && (ahead & 1) == 0;
@@ -431,7 +441,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
             fresh = any_parked = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const int head = g + 8 * r;
+                const int head = MIRROR ? g & 3 : g + 8 * r;
                 const T* qrow = reinterpret_cast<const T*>(p.q) + (row_of(cur.list) + (head < heads ? head : 0)) * D;
                 float f[KS][4], top = 0.f;
 #pragma unroll
@@ -597,7 +607,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                     }
                 exponents();
             }
-            uint32_t pb[NR][2], pl[NR][2];
+            uint32_t pb[NR][2], pl[NR][2];                               // first and second terms (MIRROR: both in pb)
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 float w[4];
@@ -608,8 +618,9 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
-                    pb[r][i] = transpose8x8(hi);
-                    pl[r][i] = transpose8x8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi, QS ? 0x1p12f : 1.f));
+                    const uint32_t rest = pack_f16_rest(w[2 * i], w[2 * i + 1], hi, QS || MIRROR ? 0x1p12f : 1.f);
+                    pb[r][i] = transpose8x8(MIRROR && t >= 2 ? rest : hi);
+                    if (!MIRROR) pl[r][i] = transpose8x8(rest);
                 }
             }
             // ---- O^T += V^T P^T
@@ -636,7 +647,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t low[4] = {a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1]};      // operand of the second terms
-                    if (QS) {
+                    if (QS && !MIRROR) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) low[i] = shift_down(low[i]);
                     }
@@ -644,14 +655,18 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
                     for (int r = 0; r < NR; ++r) {
                         if (QS && !park) {
                             float part[4];
-                            mma_f16_fresh(part, low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
-                            mma_f16(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
+                            if (MIRROR) {
+                                mma_f16_fresh(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
+                            } else {
+                                mma_f16_fresh(part, low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
+                                mma_f16(part, a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
+                            }
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[r][2 * w + e][i] += part[i];
                             continue;
                         }
                         mma_f16(o[r][2 * w + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[r][0], pb[r][1]);
-                        mma_f16(o[r][2 * w + e], low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
+                        if (!MIRROR) mma_f16(o[r][2 * w + e], low[0], low[1], low[2], low[3], pl[r][0], pl[r][1]);
                     }
                 }
             }
@@ -662,6 +677,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
         const int done = t0 + (it >> 1) + 1;
         if (!(it & 1) || (done != cur.next && done != t1) || p.solo) continue;
         unpark();
+        fold();
         const bool whole = done == cur.next && t0 <= cur.first;
         const int range = cta * TG + tg;
         const size_t part = ((size_t)unit * (p.ranges + p.lists) + range + cur.list) * p.rows;
@@ -697,6 +713,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, R2 && (sizeof(T) == 4 || D == 
 
     // ---- solo: the warps of a unit merge through shared memory, o relative to m
     unpark();
+    fold();
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem);                          // [warps][rows][D]
 #pragma unroll
@@ -843,25 +860,26 @@ __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ 
     if (threadIdx.x == 0) TIDAL_STAMP(10);
 }
 
-template <typename T, int D, bool R2>
+template <typename T, int D, int H>
 static int launch_one_kv8(const AttnKv8Params& p, cudaStream_t st) {
+    constexpr bool R2 = H == 16;
     const size_t smem = Kv8Ring<D, R2>::bytes + (p.ragged && !p.solo ? sizeof(int) * (p.lists + 1) : 0);
     // the limit is set to the most that a call may need, once per device (the call costs half a microsecond)
     static std::atomic<uint64_t> set{0};
     int dev = 0;
     TIDAL_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1u)) {
-        TIDAL_CUDA_OK(cudaFuncSetAttribute(attn_kv8_kernel<T, D, R2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        TIDAL_CUDA_OK(cudaFuncSetAttribute(attn_kv8_kernel<T, D, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)(Kv8Ring<D, R2>::bytes + sizeof(int) * (kKv8MaxPrefix + 1))));
         if (dev < 64) set.fetch_or((uint64_t)1 << dev);
     }
-    TIDAL_CUDA_OK(launch_pdl(attn_kv8_kernel<T, D, R2>, dim3((unsigned)p.slices * (unsigned)p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
+    TIDAL_CUDA_OK(launch_pdl(attn_kv8_kernel<T, D, H>, dim3((unsigned)p.slices * (unsigned)p.ctas), dim3(kKv8Warps * 32), smem, st, 1, p));
     count_launch();
     return TIDAL_OK;
 }
 template <typename T, int D>
 static int launch_attn_kv8(const AttnKv8Params& p, cudaStream_t st) {
-    const int rc = p.rows > 8 ? launch_one_kv8<T, D, true>(p, st) : launch_one_kv8<T, D, false>(p, st);
+    const int rc = p.rows > 8 ? launch_one_kv8<T, D, 16>(p, st) : p.rows > 4 ? launch_one_kv8<T, D, 8>(p, st) : launch_one_kv8<T, D, 4>(p, st);
     if (rc != TIDAL_OK || p.solo || p.ranges == 1) return rc;
     const int64_t heads = (int64_t)p.lists * (p.per_head ? 1 : p.Hq);
     const int split = p.ranges >= 16 * (int64_t)p.lists ? 8 : p.ranges >= 4 * (int64_t)p.lists ? 4 : 1;
