@@ -277,3 +277,21 @@ def test_attention_long_sums_of_ordinary_weights(T, Hq, D):
         off = (o[b:b + 20].view(-1, D) - want).norm(dim=1) / size
         worst = max(worst, float((off / tol).max()))
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("Hq,D", [(8, 64), (8, 128), (3, 128), (12, 64)])
+def test_attention_of_one_token_is_its_value(T, Hq, D):
+    """fp32, one token: the result is its value whatever the logit.  The weight and the denominator are the same exponential of
+    the same argument, 2^(x - m), but for powers of two; what differs is the weight's two terms (2^-22), the division, the
+    product with it and the scaling (2^-24 each), one to spare."""
+    g = _gen(D + Hq)
+    B = 64
+    kv, sc = T.alloc_kv8(B, 1, 1, D)
+    k, v = torch.randn(B, 1, D, generator=g).cuda(), torch.randn(B, 1, D, generator=g).cuda()
+    T.append_kv8(k, v, kv, sc, batch=B)
+    ws = T.Workspace(B, Hq, D, 1, 1)
+    q = (3 * torch.rand(B, Hq, 1, generator=g) * torch.randn(B, Hq, D, generator=g)).cuda()
+    o = T.decode_attention_kv8(q, kv, sc, 1, ws).cpu().double()
+    want = K8.values(kv.cpu(), sc.cpu())[:, 1, 0]                                    # [B, 1, D]
+    assert ws.status() == 0
+    assert ((o - want).abs() <= (2.0 ** -22 + 4 * 2.0 ** -24) * want.abs()).all(), float(((o - want).abs() / want.abs().clamp(min=1e-30)).max().log2())

@@ -240,6 +240,7 @@ __device__ __forceinline__ int range_of(int i, int total, int ranges) { return (
 template <typename T, int D, int H>      // H: query heads to a unit, at most: 4, 8 or 16
 __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || D == 128) ? 1 : 2) attn_kv8_kernel(const __grid_constant__ AttnKv8Params p) {
     constexpr bool QS = sizeof(T) == 4, R2 = H == 16, MIRROR = H == 4;
+    constexpr float kBinades = QS ? 0.f : 14.f;                          // of the weights' range that M leaves to the exponent
     constexpr int S = Kv8Ring<D, R2>::stages, KC = D / 64, KS = D / 16, VB = D / 8, NR = R2 ? 2 : 1;
     constexpr bool park = QS && D == 128 && !R2;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -541,11 +542,12 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
                             p.scores[(row_of(cur.list) + head) * p.score_stride + i0 + (i >> 1) * 8] = sf[r][i] * (kf[i >> 1] * qn2[r][i & 1]) * kLn2;
                     }
             }
-            // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M for the weights (M is kept less
-            //      the 14 binades of the weights' range)
+            // ---- exponents of the sums: xl = x - m for the denominator, xw = x + ev - M for the weights.  M is kept less
+            //      the 14 binades of the weights' range; where the result is fp32 they are a factor behind the exponential, so
+            //      that the argument of a heavy token's is small and rounded finely (2^-21 of a weight otherwise)
             float xl[NR][4], xw[NR][4];
             auto exponents = [&]() -> bool {
-                float top = 0.f, topw = 14.f;
+                float top = 0.f, topw = kBinades;
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
                         top = fmaxf(top, xl[r][i]);
                         topw = fmaxf(topw, xw[r][i]);
                     }
-                return top > 0.f || topw > 14.f;
+                return top > 0.f || topw > kBinades;
             };
             if (__any_sync(0xffffffffu, exponents())) {
 #pragma unroll
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
                             topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
                         }
-                        const float mn = fmaxf(m[r][e], ceilf(top)), Mn = fmaxf(M[r][e], ceilf(topv) - 14.f);
+                        const float mn = fmaxf(m[r][e], ceilf(top)), Mn = fmaxf(M[r][e], ceilf(topv) - kBinades);
                         l[r][e] *= fast_exp2(m[r][e] - mn);
                         const float a = fast_exp2(M[r][e] - Mn);
                         m[r][e] = mn;
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
                 l[r][0] += fast_exp2(xl[r][0]) + fast_exp2(xl[r][2]);
                 l[r][1] += fast_exp2(xl[r][1]) + fast_exp2(xl[r][3]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = fast_exp2(xw[r][i]);
+                for (int i = 0; i < 4; ++i) w[i] = QS ? fast_exp2(xw[r][i]) * 0x1p14f : fast_exp2(xw[r][i]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
@@ -690,7 +692,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                 if (head >= heads) continue;
-                Pow2 f(M[r][e] - m[r][e]);
+                Pow2 f(M[r][e] + (kBinades - 14.f) - m[r][e]);
                 if (whole) f.b *= sum == 0.f ? 0.f : 1.f / sum;
                 const size_t out = row_of(cur.list) + head;
                 if (g == 0) {
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
                 ml[warp][head][0] = m[r][e];
                 ml[warp][head][1] = sum;
             }
-            const Pow2 f(M[r][e] - m[r][e]);
+            const Pow2 f(M[r][e] + (kBinades - 14.f) - m[r][e]);
             float* at = so + ((size_t)warp * p.rows + head) * D + g * VB;
 #pragma unroll
             for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(at + 2 * j) = make_float2(f.times(o[r][j][e]), f.times(o[r][j][2 + e]));
