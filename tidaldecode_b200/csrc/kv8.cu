@@ -110,7 +110,7 @@ __device__ __forceinline__ void values8(uint2 c, float* x) {
 // single row, every group of D/8 lanes takes its own (ONE).  Up to eight (32-bit rows: four) row steps stay in registers between the pass that
 // finds the maximum and the one that writes codes, with all their loads in flight at once; longer blocks read the rows
 // behind those a second time (from L2).  Bound by HBM: 16-bit rows in, 8-bit codes out.  32 K tokens x 32 heads x 128, fp16,
-// blocks of 16: 151 us for 805 MB, 5.3 TB/s (176 us while the rows waited for the page lookup).
+// blocks of 16: 158 us for 805 MB, 5.1 TB/s (a sixth more while the rows waited for the page lookup).
 template <typename T, int D, bool ONE>
 __global__ void __launch_bounds__(256) append_kv8_kernel(const AppendKv8Params p) {
     constexpr int LPR = D / 8, RPW = 32 / LPR;
@@ -219,7 +219,7 @@ struct ReadKv8Params {
 };
 
 // A thread keeps its plane, head and 16 elements and walks over tokens, kReadSteps of them with their loads in flight together.
-// Bound by HBM: 32 K tokens x 32 heads x 128 to fp16, 133 us for 805 MB, 6.0 TB/s.  With all indices formed anew per vector it
+// Bound by HBM: 32 K tokens x 32 heads x 128 to fp16, 131 us for 805 MB, 6.1 TB/s.  With all indices formed anew per vector it
 // was bound by instructions (310 for 16 codes, 158 us).
 constexpr int kReadSteps = 2;
 template <typename T, int D>

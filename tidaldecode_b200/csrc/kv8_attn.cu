@@ -24,8 +24,8 @@
 // 8e-6 of a result after 30 K tokens, 1.7e-5 after 7 K tokens to a warp).  So where the result is fp32 the chain is short, and
 // what it gives is added by ordinary additions: after every tile where registers allow, after kKv8Chain tiles, with
 // the sums in local memory, where they do not (D = 128, up to eight heads to a unit).  8 sequences, one head to a unit, 8192
-// tokens, D = 128: 38.6 us unsplit, 53 after every tile (spills), 39.3 parked; 16 heads to a unit, 16384 tokens, D = 64: 27.6,
-// 28.0, 30.8.  For 16-bit results the rounding of the result is a hundred times larger, and the chain stays whole.
+// tokens, D = 128: 38.7 us unsplit, 43.1 after every tile (spills), 38.8 parked; 16 heads to a unit, 16384 tokens, D = 64: 28.0,
+// 28.4, 31.4.  For 16-bit results the rounding of the result is a hundred times larger, and the chain stays whole.
 //
 // Data movement.  Every warp has a ring of tiles of its own in shared memory, filled with cp.async, 16 bytes to a lane and a
 // whole row to adjacent lanes (with the two pieces of a 32-byte sector four lanes apart, sectors were fetched twice: 6.0
@@ -40,10 +40,12 @@
 // Both products have the few query heads as N: with heads as M (16 rows, most of them zero) the first took twice the
 // instructions and twice the registers.  A lane's accumulators belong to heads 2t and 2t+1 throughout.
 //
-// Bound by HBM on long contexts: 64 sequences of 16 K tokens, 32/8 heads of 128 (2.1 GB) 331 us, 6.5 TB/s; 16 of them 93 us
-// (5.8 TB/s), of which 6 us pass before the first tile is there, 7 between the first and the last warp's end and 3 in the merge.
+// Bound by HBM on long contexts: 64 sequences of 16 K tokens, 32/8 heads of 128 (2.1 GB) 334 us, 6.5 TB/s; 16 of them 95 us
+// (5.7 TB/s), of which 6 to 8 us pass before the first tile is there, 16 between the first and the last CTA's end and 5 in the
+// merge.
 // The same tile loop on the tensor cores' 5th-generation instructions has no use here: at most 16 query rows share a K tile
-// (a tile of tcgen05.mma has 64), and removing either product altogether does not change the time.
+// (a tile of tcgen05.mma has 64), and removing either product altogether takes nothing off (95 us: 94) or, of 32 K tokens with
+// logits, 4 of 58 us.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -60,8 +62,8 @@ constexpr int kKv8Tile = 16;             // tokens a warp takes at a time; it lo
 constexpr int kKv8Pair = 2 * kKv8Tile;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kKv8MaxPrefix = 2048;      // lists whose lengths a CTA adds up itself; beyond, a CTA per list
-// Lists up to this long go to a CTA each.  One sequence of 256 / 512 / 1024 tokens, 8 KV heads: 6.2 / 8.5 / 12.9 us that way, 8.2 /
-// 8.1 / 8.5 us in ranges and a merge.
+// Lists up to this long go to a CTA each.  One sequence of 256 / 512 / 1024 tokens, 8 KV heads: 6.5 / 8.8 / 13.0 us that way, 8.6 /
+// 8.6 / 9.0 us in ranges and a merge.
 constexpr int kKv8SoloTokens = 384;
 
 struct AttnKv8Params {
@@ -765,8 +767,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, H == 16 && (sizeof(T) == 4 || 
 // heads, `split` warps to a head; where there are few heads only blockIdx.y's 32 elements of them, four parts to a warp at a
 // time (one list of 256 K tokens: 10 us less).  What depends on lengths and launch alone is worked out before the attention
 // kernel has ended; then a part costs one trip to L2: each group of lanes keeps a maximum of its own.  (The lengths were
-// there before that kernel began: it waits for its predecessor before it lets this one start.)  Bound by latency, 1.5 to 3
-// us behind the attention kernel.
+// there before that kernel began: it waits for its predecessor before it lets this one start.)  Bound by latency: done 3
+// to 5 us after the last CTA of the attention kernel (7 where 64 ragged sequences' lengths are added up), 7.5 us alone and cold.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) merge_kv8_kernel(const __grid_constant__ AttnKv8Params p, int split) {
     extern __shared__ int prefix_m[];                    // [lists + 1], ragged
